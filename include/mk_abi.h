@@ -69,7 +69,8 @@ int mk_launch_params(const MkLaunch* launch, char* text, uint64_t cap_bytes);
 // host (synchronises the stream first). code 0 = clean; otherwise the wait that gave up.
 typedef struct MkLaunchStatus {
     int64_t code;      // 0 ok, 1 an exchange wait ran out (a peer never signalled), 3 a bulk copy or tensor-core barrier
-                       // never completed, 4 an out-of-range position / request index was clamped, 6 a row's router
+                       // never completed, 4 an out-of-range position / request index was clamped, 5 a batched step
+                       // found no room for its rows or pages, 6 a row's router
                        // scores were NaN (it is routed to the lowest expert ids; its outputs are meaningless)
     int64_t stage;     // stage index that recorded it (exchange waits), or a kernel-specific site number
     int64_t block;     // blockIdx.x
@@ -670,6 +671,161 @@ typedef struct MkDflashKvSyncBind {
     uint64_t status;
 } MkDflashKvSyncBind;
 int mk_dflash_kv_sync_bind(MkModule* module, const MkDflashKvSyncBind* bind, MkLaunch** out);
+
+// ---- the cache path of a batched step ----------------------------------------------------------------------------------------
+// No counterpart in the reference, whose step is one request's (abi.h:213-239). Four launches for a batch of requests on one
+// paged K/V pool, in the order a step runs them: pages and slots for the new tokens, the rope table (once), the rotation with
+// its K/V append, and the attention. A pool row ("slot") is page x page_size + offset; page size 1 makes the page table the
+// framework's token-granular request table. All lengths are read on the device, so a captured launch follows the batch; rows
+// behind the step's last token are left as they were. A launch's outputs and scratch are its own: it may not overlap itself
+// on two streams (bind it twice for that). `status` (i32 [16] or 0) records what was left out: code 4 an index or length that
+// contradicts the extents, 5 a step that found no room, 3 a copy or tensor-core barrier that never completed.
+// Device pointers have to lie on the module's device; mk_launch switches to that device for the call where another is current.
+
+// Block tables and slot maps. need = ceil((seq_lens + new_lens) / page_size) pages a request; those it does not own yet come
+// from the ring of free pages, request by request. A request with seq_lens = new_lens = 0 is padding (its index is not read).
+// Left out, with status code 4: negative or overlong lengths, an index outside the pool, a pool row that two requests name (all
+// of them), fewer owned pages than its tokens fill. They count as padding. When the rows or the free pages do not cover the
+// whole step nobody gets any (status code 5): cu_rows is 0 throughout and kv_lens is seq_lens.
+typedef struct MkBlockTablesBind {
+    uint64_t seq_lens;          // i64 [batch]: tokens in the cache
+    uint64_t new_lens;          // i64 [batch]: tokens to come
+    uint64_t req_pool_indices;  // i64 [batch]: rows of req_to_page
+    uint64_t req_to_page;       // i32 [pool_rows, width], read and extended
+    int64_t pool_rows;
+    int64_t width;
+    uint64_t pages_owned;       // i32 [pool_rows], read and advanced
+    uint64_t free_pages;        // i32 [ring]: page ids; entry w % ring for words head <= w < tail
+    int64_t ring;
+    uint64_t free_words;        // i64 [2] {head, tail}: head advances by the pages taken; pages are given back by writing
+                                // them behind the tail and advancing it, between launches
+    int64_t page_size;
+    int64_t batch;
+    int64_t rows;               // capacity of slots / positions
+    uint64_t block_table;       // out i32 [batch, width]: pages 0 .. need - 1, then -1
+    uint64_t slots;             // out i64 [rows]: pool row of each new token
+    uint64_t positions;         // out i64 [rows]
+    uint64_t cu_rows;           // out i32 [batch + 1]: first row of each request
+    uint64_t kv_lens;           // out i32 [batch]: seq_lens + new_lens
+    uint64_t ticket;            // u32 [1], zeroed once by the caller
+    uint64_t status;
+} MkBlockTablesBind;
+int mk_block_tables_bind(MkModule* module, const MkBlockTablesBind* bind, MkLaunch** out);
+
+// Rope table: out[r] = {cos(a_0) .. | sin(a_0) ..} x mult, a_i = (first + r) f_i, angles in 64 bits. f_i = theta^(-2i / rot), then
+//   kind 0 as it is; 1 linear: f / factor; 2 ntk: theta x factor^(rot / (rot - 2));
+//   3 llama3: f / factor below low_freq_factor turns in original_len, f above high_freq_factor turns, blended linearly in the
+//     turns between; 4 yarn: from f (dims that turn more than beta_fast times in original_len) to f / factor (less than
+//     beta_slow) along a ramp over the dims, mult = 0.1 ln(factor) + 1 (1 for factor <= 1). mult is 1 for the others.
+typedef struct MkRopeTableBind {
+    uint64_t out;    // f32 [rows, rot]
+    int64_t rows;
+    int64_t first;   // position of row 0
+    int64_t rot;     // multiple of 8, up to 256
+    double theta;    // > 1
+    int64_t kind;
+    double factor;
+    double low_freq_factor;
+    double high_freq_factor;
+    double beta_fast;
+    double beta_slow;
+    double original_len;
+} MkRopeTableBind;
+int mk_rope_table_bind(MkModule* module, const MkRopeTableBind* bind, MkLaunch** out);
+
+// Rotation of q and k by position, with the append of k and v. Strides are in elements; 16-byte aligned heads. q_out may be q
+// and k_out may be k (in place); other overlaps are not allowed. A row with a negative slot is rotated and not appended; the
+// slots of a step's rows differ. A position outside the table or a slot outside the pool is recorded (code 4): row 0 of
+// the table stands in for the position, the row is not appended.
+typedef struct MkRotaryBind {
+    uint64_t q;              // bf16 or f16 [rows, q_heads, head_dim]
+    int64_t q_row;
+    int64_t q_head;
+    uint64_t k;              // [rows, kv_heads, head_dim] (0 with kv_heads 0)
+    int64_t k_row;
+    int64_t k_head;
+    uint64_t v;              // as k, or 0: no append of v
+    int64_t v_row;
+    int64_t v_head;
+    uint64_t q_out;
+    int64_t qo_row;
+    int64_t qo_head;
+    uint64_t k_out;          // rotated k rows, or 0
+    int64_t ko_row;
+    int64_t ko_head;
+    uint64_t positions;      // i64 [rows]
+    uint64_t cos_sin_cache;  // f32 [cos_sin_rows, rot] {cos | sin}
+    int64_t cos_sin_rows;
+    uint64_t slots;          // i64 [rows] (needed with k_cache)
+    uint64_t k_cache;        // [kv_rows, kv_heads, head_dim], or 0: no append
+    int64_t kc_row;
+    int64_t kc_head;
+    uint64_t v_cache;
+    int64_t vc_row;
+    int64_t vc_head;
+    int64_t kv_rows;
+    uint64_t n_rows;         // i32 [1] live rows, or 0: all
+    int64_t rows;
+    int64_t q_heads;
+    int64_t kv_heads;
+    int64_t head_dim;        // multiple of 8, up to 256
+    int64_t rot;             // rotated dims: multiple of 8, up to head_dim
+    int64_t interleaved;     // 0: pairs (i, i + rot / 2), 1: pairs (2i, 2i + 1)
+    int64_t inverse;         // 1: rotates back (also the gradient of the rotation)
+    int64_t fp16;            // 0: bf16, 1: f16
+    uint64_t status;
+} MkRotaryBind;
+int mk_rotary_bind(MkModule* module, const MkRotaryBind* bind, MkLaunch** out);
+
+// Attention of a batch's new rows over the paged cache. Request b's rows are [cu_rows[b], cu_rows[b + 1]), the last of its
+// kv_lens[b] keys; its row at position x sees the keys max(0, x - window) .. x (window 0: all up to x). The first prefix_len keys
+// are the same cache rows for every request (their block-table rows begin alike) and are read once for the whole batch; a
+// request shorter than that sees its own length of them. A row that sees no key is 0 with lse -inf. Softmax statistics and sums
+// are f32; the probabilities are rounded to the inputs' type for the product with V. A NaN or infinity in a K or V row that
+// some row of the batch sees through the same tile may reach the other rows of that tile; cache rows that no request's
+// table and length name are never read. Page ids outside the pool are recorded (code 4) and read as zero rows.
+typedef struct MkPrefixAttnBind {
+    uint64_t q;            // bf16 or f16 [rows, q_heads, head_dim]
+    int64_t q_row;         // strides in elements, multiples of 8
+    int64_t q_head;
+    uint64_t k_cache;      // [kv_rows, kv_heads, head_dim]
+    int64_t k_row;
+    int64_t k_head;
+    uint64_t v_cache;
+    int64_t v_row;
+    int64_t v_head;
+    int64_t kv_rows;
+    uint64_t block_table;  // i32 [batch, width]
+    int64_t table_row;     // entries between its rows
+    int64_t width;
+    uint64_t kv_lens;      // i32 [batch]
+    uint64_t cu_rows;      // i32 [batch + 1]
+    uint64_t prefix_len;   // i32 [1]
+    uint64_t out;          // [rows, q_heads, head_dim]
+    int64_t o_row;
+    int64_t o_head;
+    uint64_t lse;          // f32 [rows, q_heads] natural log of the softmax sum, or 0
+    int64_t rows;          // capacity of q / out
+    int64_t batch;
+    int64_t max_new;       // largest number of rows of a request
+    int64_t q_heads;
+    int64_t kv_heads;
+    int64_t head_dim;      // 64 or 128
+    int64_t page_size;
+    int64_t window;
+    double scale;
+    int64_t fp16;
+    uint64_t ws;           // ws_bytes of scratch (mk_prefix_attn_constants), 256-byte aligned
+    int64_t ws_bytes;
+    uint64_t status;
+} MkPrefixAttnBind;
+typedef struct MkPrefixAttnConstants {
+    int64_t ws_bytes;
+    int64_t ctas;     // CTAs that share the work
+    int64_t kernels;  // kernels per launch
+} MkPrefixAttnConstants;
+int mk_prefix_attn_constants(const MkPrefixAttnBind* bind, MkPrefixAttnConstants* out);
+int mk_prefix_attn_bind(MkModule* module, const MkPrefixAttnBind* bind, MkLaunch** out);
 
 #ifdef __cplusplus
 }

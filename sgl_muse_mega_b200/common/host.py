@@ -82,7 +82,8 @@ EXPORTS = (
     "mk_qkv_launch_static", "mk_feeds_bind", "mk_entry_bind", "mk_lm_head_bind", "mk_softcap_bind", "mk_accept_bind",
     "mk_symm_alloc", "mk_symm_open", "mk_symm_close", "mk_symm_free", "mk_dflash_constants", "mk_dflash_entry_bind",
     "mk_dflash_layer_bind", "mk_dflash_draft_head_bind", "mk_dflash_kv_sync_bind", "mk_dflash_tree_bind",
-    "mk_dflash_tree_compact_bind",
+    "mk_dflash_tree_compact_bind", "mk_block_tables_bind", "mk_rope_table_bind", "mk_rotary_bind", "mk_prefix_attn_constants",
+    "mk_prefix_attn_bind",
 )  # fmt: skip
 
 
@@ -112,8 +113,11 @@ class Library:
         d.mk_qkv_bind.argtypes = [vp, P(STRUCTS["MkQkvBind"]), P(vp)]
         d.mk_qkv_launch_static.argtypes = [P(STRUCTS["MkQkvBind"]), ctypes.c_uint64]
         for fn, st in (("mk_feeds_bind", "MkFeedsBind"), ("mk_entry_bind", "MkEntryBind"), ("mk_lm_head_bind", "MkLmHeadBind"),
-                       ("mk_softcap_bind", "MkSoftcapBind"), ("mk_accept_bind", "MkAcceptBind")):  # fmt: skip
+                       ("mk_softcap_bind", "MkSoftcapBind"), ("mk_accept_bind", "MkAcceptBind"),
+                       ("mk_block_tables_bind", "MkBlockTablesBind"), ("mk_rope_table_bind", "MkRopeTableBind"),
+                       ("mk_rotary_bind", "MkRotaryBind"), ("mk_prefix_attn_bind", "MkPrefixAttnBind")):  # fmt: skip
             getattr(d, fn).argtypes = [vp, P(STRUCTS[st]), P(vp)]
+        d.mk_prefix_attn_constants.argtypes = [P(STRUCTS["MkPrefixAttnBind"]), P(STRUCTS["MkPrefixAttnConstants"])]
         d.mk_dflash_constants.argtypes = [P(STRUCTS["MkDflashShape"]), P(STRUCTS["MkDflashConstants"])]
         for fn, st in (("mk_dflash_entry_bind", "MkDflashEntryBind"), ("mk_dflash_layer_bind", "MkDflashLayerBind"),
                        ("mk_dflash_draft_head_bind", "MkDflashDraftHeadBind")):  # fmt: skip
@@ -163,12 +167,18 @@ class Library:
 
 
     def bind(self, fn_name: str, module: "Module | None", bind) -> "Launch":
-        """Any ``mk_*_bind(module, bind, out)`` entry point by name (feeds, entry, lm_head, softcap, accept)."""
+        """Any ``mk_*_bind(module, bind, out)`` entry point by name (feeds, entry, lm_head, softcap, accept, the batched
+        step's tables, rotation and attention)."""
         out = ctypes.c_void_p()
         fn = getattr(self.dll, fn_name)
         self.check(fn(module.handle if module else None, ctypes.byref(bind), ctypes.byref(out)), fn_name)
         return Launch(self, out, module)
 
+
+    def prefix_attn_constants(self, bind) -> ctypes.Structure:
+        c = STRUCTS["MkPrefixAttnConstants"]()
+        self.check(self.dll.mk_prefix_attn_constants(ctypes.byref(bind), ctypes.byref(c)), "mk_prefix_attn_constants")
+        return c
 
     def dflash_constants(self, shape) -> ctypes.Structure:
         c = STRUCTS["MkDflashConstants"]()

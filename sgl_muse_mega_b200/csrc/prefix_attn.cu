@@ -1,0 +1,839 @@
+// Attention of a batch's new rows over a paged K/V cache whose first tokens all requests share.
+//
+//   out[t, h] = sum_k p_k V[k] / sum_k p_k,  p_k = exp(scale q[t, h] . K[k]),  k over the keys that row t sees:
+//   the row at position x of request b sees the keys max(0, x - window) .. x (window 0: 0 .. x), x = kv_len - new + its index
+//
+// The keys below prefix_len are the same cache rows for every request, so they are visited once for all of them: the
+// query rows of the whole batch (tokens x the G query heads of a kv head) stand in one tall operand, and a K / V tile that
+// was brought in serves 256 of them. The keys behind the prefix are visited per request. Softmax pieces (m, l, O) over
+// disjoint key sets merge exactly, so any split of the work gives the same result up to f32 rounding.
+//
+// Work. An item is (kv head, block of up to 256 rows, its key tiles of 128): first the prefix items, then each request's
+// own. A step is one 128-row x 128-key tile product: an item of more than 128 rows takes two steps a key tile (its two
+// row halves), one of at most 128 rows takes one. All items' steps form one sequence that is cut evenly over the CTAs
+// (one an SM), whatever the lengths; they are read on the device, so a captured launch follows the batch. The piece of
+// item i that CTA c computes goes to slot i + c of the scratch: walking the sequence, every new piece moves to the next
+// item or the next CTA, so the slots are distinct. prefix_merge_kernel adds the pieces of each row, in slot order.
+//
+// A CTA's twelve warps: two softmax warpgroups (a thread holds one query row, its scores are one TMEM lane), one thread
+// that issues the tensor-core products, a warp that gathers K and V rows (TMA gather of four cache rows a lane, so any
+// page size costs the same), two that gather the queries. Steps alternate between the two warpgroups, each with its own
+// S, P and O in tensor memory: while one takes the exponentials of its step the tensor core works for the other.
+#include "batch.h"
+#include "umma.cuh"
+#include "util.cuh"
+
+namespace mk {
+
+using namespace umma;
+
+constexpr int kTile = 128;  // rows of a step and keys of a tile
+constexpr int kAttnThreads = 384;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// ---- the plan: the same numbers in every warp of both kernels ---------------------------------------------------------
+struct PlanHead {  // in front of the scratch, for the merge kernel
+    unsigned total, prefix_steps, tiles, row_blocks, per_head, p_lo, prefix, tokens;
+};
+
+struct Req {
+    int first, n, len;  // its first row, its rows, its keys
+};
+// the lengths of request b as far as they are usable: what contradicts the launch's extents is left out (and recorded)
+__device__ __forceinline__ Req request(const PrefixAttnArgs& a, int b, int* status) {
+    Req r;
+    r.first = __ldg(a.cu_rows + b);
+    r.n = __ldg(a.cu_rows + b + 1) - r.first;
+    r.len = __ldg(a.kv_lens + b);
+    const long long cap = (long long)a.width * a.page;
+    if (r.n < 0 || r.n > a.max_new || r.first < 0 || r.first + r.n > a.rows) {
+        if (status != nullptr) batch_status(status, 4, 520, b, r.n);
+        r.n = 0;
+    }
+    if (r.len < 0 || r.len > cap) {
+        if (status != nullptr) batch_status(status, 4, 521, b, r.len);
+        r.n = 0;
+    }
+    return r;
+}
+// steps of one key tile over all row blocks of `rows` rows: two for every 256 rows, one for a rest of up to 128
+__device__ __forceinline__ unsigned steps_of_rows(int rows) { return (unsigned)((rows + kTile - 1) / kTile); }
+__device__ __forceinline__ int own_first(const PrefixAttnArgs& a, const Req& r, int prefix) {  // first key of its own tiles
+    const int lo = a.window > 0 ? max(0, r.len - r.n - a.window) : 0;
+    return max(prefix, lo);
+}
+__device__ __forceinline__ unsigned own_tiles(const PrefixAttnArgs& a, const Req& r, int prefix) {
+    const int k0 = own_first(a, r, prefix);
+    return r.n > 0 && r.len > k0 ? (unsigned)(r.len - k0 + kTile - 1) / kTile : 0u;
+}
+__device__ __forceinline__ unsigned own_steps(const PrefixAttnArgs& a, const Req& r, int prefix) {
+    return own_tiles(a, r, prefix) * steps_of_rows(r.n * a.G) * a.kvh;
+}
+__device__ __forceinline__ int row_blocks(int rows) { return (rows + 2 * kTile - 1) / (2 * kTile); }
+__device__ __forceinline__ int own_items(const PrefixAttnArgs& a, const Req& r) { return row_blocks(r.n * a.G) * a.kvh; }
+
+struct Plan {
+    int prefix;         // shared keys (0: none shared)
+    int p_lo;           // first shared key that any row sees
+    int ref;            // the request whose table row names the shared pages
+    int tokens;         // rows of the batch
+    unsigned tiles;     // key tiles of a prefix item
+    unsigned per_head;  // steps of a kv head's prefix items
+    unsigned prefix_steps, total;
+};
+
+// One warp; every lane gets the result. Three passes over the batch's lengths, which stay in L1.
+__device__ Plan make_plan(const PrefixAttnArgs& a, int lane, int* status, unsigned* cum) {
+    Plan p;
+    const int cap = (int)min((long long)a.width * a.page, 0x7fffffffll);
+    int want = __ldg(a.prefix_len);
+    if (want < 0 || want > cap) {
+        if (status != nullptr) batch_status(status, 4, 522, want, cap);
+        want = 0;
+    }
+    p.tokens = __ldg(a.cu_rows + a.batch);
+    if (p.tokens < 0 || p.tokens > a.rows) {
+        if (status != nullptr) batch_status(status, 4, 523, p.tokens, a.rows);
+        p.tokens = 0;
+    }
+    int live = 0, ref = 0x7fffffff, lo = 0x7fffffff, hi = 0;
+    for (int b = lane; b < a.batch; b += 32) {
+        const Req r = request(a, b, status);
+        if (r.n <= 0 || r.len <= 0) continue;
+        ++live;
+        if (r.len >= want) ref = min(ref, b);
+        lo = min(lo, a.window > 0 ? max(0, r.len - r.n - a.window) : 0);
+        hi = max(hi, min(want, r.len));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        live += __shfl_xor_sync(0xffffffffu, live, o);
+        ref = min(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    // one request shares with nobody, and a prefix that no request holds whole cannot be read through one table row
+    p.prefix = live > 1 && ref != 0x7fffffff ? want : 0;
+    p.ref = p.prefix > 0 ? ref : 0;
+    p.p_lo = p.prefix > 0 ? lo / kTile * kTile : 0;
+    p.tiles = p.prefix > 0 && hi > p.p_lo ? (unsigned)(hi - p.p_lo + kTile - 1) / kTile : 0u;
+    p.per_head = p.tiles * steps_of_rows(p.tokens * a.G);
+    p.prefix_steps = p.per_head * a.kvh;
+    unsigned sum = p.prefix_steps;
+    int items = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int b = b0 + lane;
+        Req r{0, 0, 0};
+        if (b < a.batch) r = request(a, b, nullptr);
+        const unsigned x = own_steps(a, r, p.prefix);
+        const int it = own_items(a, r);
+        unsigned inc = x;
+        int ci = it;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
+            const int z = __shfl_up_sync(0xffffffffu, ci, o);
+            if (lane >= o) inc += y, ci += z;
+        }
+        if (cum != nullptr && b < a.batch) {  // first step and first item of each request
+            cum[b] = sum + inc - x;
+            cum[a.batch + b] = (unsigned)(items + ci - it);
+        }
+        sum += __shfl_sync(0xffffffffu, inc, 31);
+        items += __shfl_sync(0xffffffffu, ci, 31);
+    }
+    p.total = sum;
+    return p;
+}
+
+__device__ __forceinline__ unsigned range_lo(unsigned total, int c, int ctas) { return (unsigned)((unsigned long long)total * c / ctas); }
+__device__ __forceinline__ int cta_of(unsigned step, unsigned total, int ctas) {  // whose range holds the step
+    return (int)((((unsigned long long)step + 1) * ctas - 1) / total);
+}
+
+// An item's piece in one CTA's range
+struct Piece {
+    int b;            // request, -1: the prefix
+    int h, rb;        // kv head, row block
+    int index;        // number of the item within its kind (slot = index + CTA)
+    int rows;         // rows of the block (1 .. 256)
+    int n;            // request rows (own items)
+    int first, len;   // the request's first row and keys
+    int key0;         // first key of the item's tile 0
+    unsigned t0, t1;  // key tiles [t0, t1)
+    __device__ __forceinline__ bool pair() const { return rows > kTile; }
+    __device__ __forceinline__ unsigned steps() const { return (t1 - t0) << (rows > kTile ? 1 : 0); }
+};
+
+// Walks a CTA's range of steps item by item. Every role of the CTA has its own walker with the same sequence.
+struct Walker {
+    const PrefixAttnArgs& a;
+    const Plan& p;
+    unsigned pos, end;  // steps left: [pos, end)
+    int b;              // -1 while in the prefix
+    unsigned base;      // first step of the current request's items (or 0)
+    int items;          // own items before request b
+    Req r;
+    unsigned tiles, per_head;
+    int row_total;
+
+    __device__ Walker(const PrefixAttnArgs& a_, const Plan& p_, int cta, int lane) : a(a_), p(p_) {
+        pos = range_lo(p.total, cta, a.ctas);
+        end = range_lo(p.total, cta + 1, a.ctas);
+        b = -1;
+        base = 0;
+        items = 0;
+        if (pos >= p.prefix_steps && pos < end) {  // starts in a request's items: find it, the whole warp together
+            unsigned sum = p.prefix_steps;
+            int cnt = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += 32) {
+                const int bb = b0 + lane;
+                Req q{0, 0, 0};
+                if (bb < a.batch) q = request(a, bb, nullptr);
+                const unsigned x = own_steps(a, q, p.prefix);
+                const int it = own_items(a, q);
+                unsigned inc = x;
+                int ci = it;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
+                    const int z = __shfl_up_sync(0xffffffffu, ci, o);
+                    if (lane >= o) inc += y, ci += z;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, pos < sum + inc);
+                if (hit != 0u) {
+                    const int l = __ffs(hit) - 1;
+                    b = b0 + l;
+                    base = sum + __shfl_sync(0xffffffffu, inc - x, l);
+                    items = cnt + __shfl_sync(0xffffffffu, ci - it, l);
+                    break;
+                }
+                sum += __shfl_sync(0xffffffffu, inc, 31);
+                cnt += __shfl_sync(0xffffffffu, ci, 31);
+            }
+            load();
+        }
+    }
+    __device__ __forceinline__ void load() {
+        r = request(a, b, nullptr);
+        tiles = own_tiles(a, r, p.prefix);
+        row_total = r.n * a.G;
+        per_head = tiles * steps_of_rows(row_total);
+    }
+    // the next piece, false at the end of the range
+    __device__ bool next(Piece& x) {
+        while (pos < end) {
+            unsigned off;
+            if (pos < p.prefix_steps) {
+                x.b = -1;
+                row_total = p.tokens * a.G;
+                tiles = p.tiles;
+                per_head = p.per_head;
+                off = pos;
+                x.first = 0;
+                x.n = p.tokens;
+                x.len = p.prefix;
+                x.key0 = p.p_lo;
+            } else {
+                if (b < 0) {  // out of the prefix
+                    b = 0;
+                    base = p.prefix_steps;
+                    load();
+                }
+                while (pos >= base + per_head * a.kvh) {
+                    base += per_head * a.kvh;
+                    items += row_blocks(row_total) * a.kvh;
+                    ++b;
+                    load();
+                }
+                x.b = b;
+                off = pos - base;
+                x.first = r.first;
+                x.n = r.n;
+                x.len = r.len;
+                x.key0 = own_first(a, r, p.prefix);
+            }
+            x.h = (int)(off / per_head);
+            off -= x.h * per_head;
+            x.rb = (int)(off / (2 * tiles));
+            off -= x.rb * 2 * tiles;
+            const int blocks = row_blocks(row_total);
+            x.rows = min(2 * kTile, row_total - x.rb * 2 * kTile);
+            x.index = (x.b < 0 ? 0 : items) + x.h * blocks + x.rb;
+            const int sh = x.rows > kTile ? 1 : 0;
+            const unsigned len = tiles << sh, stop = min(off + (end - pos), len);
+            x.t0 = (off + sh) >> sh;  // a range that ends inside a pair of steps leaves the pair to the range that starts it
+            x.t1 = (stop + sh) >> sh;
+            pos += stop - off;
+            if (x.t1 > x.t0) return true;
+        }
+        return false;
+    }
+};
+
+// ---- scratch ----------------------------------------------------------------------------------------------------------
+// A slot holds two parts (the row halves of a pair, or the even and odd tiles of a single); a part of R rows: O as
+// [D / 4][R] float4, then m [R] and l [R].
+__host__ __device__ constexpr long long part_bytes(int rows, int dim) { return (long long)rows * (dim + 2) * 4; }
+
+// ---- the kernel --------------------------------------------------------------------------------------------------------
+template <int D>
+struct Cfg {
+    static constexpr int kAtoms = D / 64;                 // 64-wide column blocks of a K / V tile
+    static constexpr int kTileBytes = kTile * D * 2;      // K, V or Q tile
+    static constexpr int kRing = D == 64 ? 4 : 2;         // K stages and V stages
+    static constexpr int kQ = D == 64 ? 4 : 3;            // query tiles
+    static constexpr int kSmem = (2 * kRing + kQ) * kTileBytes + 1024;
+    static constexpr bool kAlias = D == 128;              // P over S: tensor memory holds 2 x (128 + 128) columns then
+    // tensor-memory columns (512): S of each warpgroup, P, O
+    static constexpr uint32_t kS = 0, kP = D == 64 ? 256 : 0, kPStep = D == 64 ? 64 : 128, kO = D == 64 ? 384 : 256, kOStep = D;
+};
+
+struct Bars {
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[4], q_empty[4];
+    uint64_t s_full[2], p_ready[2], o_full[2], pv_done[2];
+    uint64_t drain;
+    uint32_t tmem;
+    int abort;
+};
+
+__device__ __forceinline__ void gather4(void* dst, const CUtensorMap* map, int x, int y0, int y1, int y2, int y3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y0), "r"(y1), "r"(y2), "r"(y3), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// D[128 x N] (+)= A B^T, both operands in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        :
+        : "r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// the same with A in tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        :
+        : "r"(d), "r"(at), "l"(bd), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// f32 accumulator, A and B f16 (0) or bf16 (1), A K-major, B K-major or (bit 16) N-major, M = 128
+__host__ __device__ constexpr uint32_t idesc_f16(bool half, bool b_n_major, int n) {
+    return (1u << 4) | ((half ? 0u : 1u) << 7) | ((half ? 0u : 1u) << 10) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((128u >> 4) << 24);
+}
+// V as the N-major operand: 64 columns (128 bytes, swizzled) x 8 keys form an atom of 1024 bytes; the next 8 keys follow
+// it (stride offset), the next 64 columns lie a whole tile of 128-byte rows further (leading offset)
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)((kTile * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t t, float* r) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+        "%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]),
+          "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]),
+          "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]),
+          "=r"(u[31])
+        : "r"(t));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t* u) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+        "%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]),
+        "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]),
+        "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+        : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (kHalf) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Called by whole warps; one expired wait ends every role of the CTA.
+__device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, Bars* s, int* status, int where) {
+    const bool ok = mbar_wait(bar, parity, &s->abort);
+    if (__all_sync(0xffffffffu, ok)) return true;  // the whole warp goes the same way
+    if (!ok && atomicExch(&s->abort, 1) == 0) batch_status(status, 3, where, 0, 0);
+    return false;
+}
+
+// the request and index of token t of the batch (bisection over cu_rows, which is in L1)
+__device__ __forceinline__ int request_of(const PrefixAttnArgs& a, int t) {
+    int lo = 0, hi = a.batch;  // the last b with cu[b] <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(a.cu_rows + mid) <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// the keys [lo, hi) that row `rr` of a piece sees, within the piece's keys
+__device__ __forceinline__ void row_keys(const PrefixAttnArgs& a, const Plan& p, const Piece& x, int rr, int& lo, int& hi) {
+    lo = hi = 0;
+    if (rr >= x.rows) return;
+    const int j = (x.rb * 2 * kTile + rr) / a.G;  // token of the item
+    int n = x.n, len = x.len, idx = j;
+    if (x.b < 0) {
+        const int b = request_of(a, j);
+        const Req r = request(a, b, nullptr);
+        n = r.n;
+        len = r.len;
+        idx = j - r.first;
+        if (idx >= n) return;  // a request that was left out
+    }
+    const int at = len - n + idx;  // its position
+    lo = a.window > 0 ? max(0, at - a.window) : 0;
+    hi = min(at + 1, x.b < 0 ? p.prefix : len);
+    if (hi < lo) hi = lo;
+}
+
+template <int D, bool kHalf>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    prefix_attn_kernel(const PrefixAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    typedef Cfg<D> C;
+    extern __shared__ unsigned char raw[];
+    __shared__ Bars S;
+    unsigned char* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    unsigned char* Ks = smem;
+    unsigned char* Vs = Ks + C::kRing * C::kTileBytes;
+    unsigned char* Qs = Vs + C::kRing * C::kTileBytes;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&S.k_full[i], 1);
+            mbar_init(&S.k_empty[i], 1);
+            mbar_init(&S.v_full[i], 1);
+            mbar_init(&S.v_empty[i], 1);
+            mbar_init(&S.q_full[i], 64);
+            mbar_init(&S.q_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&S.s_full[i], 1);
+            mbar_init(&S.p_ready[i], 128);
+            mbar_init(&S.o_full[i], 1);
+            mbar_init(&S.pv_done[i], 1);
+        }
+        mbar_init(&S.drain, 1);
+        S.abort = 0;
+        mbar_fence_init();
+    }
+    if (warp == 8) tmem_alloc(&S.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t*)&S.tmem;
+    griddep_wait();
+
+    unsigned* cum = (unsigned*)(a.ws + 256);
+    const bool writer = blockIdx.x == 0 && warp == 0;
+    const Plan p = make_plan(a, lane, writer ? a.status : nullptr, writer ? cum : nullptr);
+    if (writer && lane == 0)
+        *(PlanHead*)a.ws = PlanHead{p.total, p.prefix_steps, p.tiles, steps_of_rows(p.tokens * a.G), p.per_head, (unsigned)p.p_lo, (unsigned)p.prefix,
+                                    (unsigned)p.tokens};
+    Walker walk(a, p, blockIdx.x, lane);
+    Piece x;
+    const int cap = a.width * a.page;
+    unsigned k_issued = 0, v_issued = 0;  // warp 9: tiles requested
+
+    if (warp < 8) {
+        // ---- softmax ----
+        const int wg = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes in bits 16 ..
+        const uint32_t tS = tmem + lanes + C::kS + wg * 128, tP = tmem + lanes + C::kP + wg * C::kPStep, tO = tmem + lanes + C::kO + wg * C::kOStep;
+        unsigned g = 0;  // steps of earlier pieces
+        uint32_t s_par = 0, o_par = 0;
+        bool ok = true;
+        while (ok && walk.next(x)) {
+            const unsigned ns = x.steps(), sub = (wg - g) & 1;
+            g += ns;
+            if (sub >= ns) continue;
+            const bool pair = x.pair();
+            const int rr = row + (pair ? (int)sub * kTile : 0);
+            const bool busy = (rr & ~31) < x.rows;  // this warp has rows
+            int lo, hi;
+            row_keys(a, p, x, rr, lo, hi);
+            float m = -INFINITY, l = 0.f;
+            for (unsigned st = sub; st < ns; st += 2) {
+                const int kb = x.key0 + (int)(x.t0 + (pair ? st >> 1 : st)) * kTile;
+                if (!(ok = attn_wait(&S.s_full[wg], s_par, &S, a.status, 530))) break;
+                s_par ^= 1;
+                if (busy) {
+                    tc_fence_after();
+                    float s[128];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_ld32(tS + 32 * i, s + 32 * i);
+                    tmem_ld_wait();
+                    if (!__all_sync(0xffffffffu, (lo <= kb && hi >= kb + kTile) || rr >= x.rows)) {
+                        const int c0 = lo - kb, c1 = hi - kb;
+#pragma unroll
+                        for (int i = 0; i < 128; ++i) s[i] = i >= c0 && i < c1 ? s[i] : -INFINITY;
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 128; i += 4) {
+                        mx[0] = fmaxf(mx[0], s[i]);
+                        mx[1] = fmaxf(mx[1], s[i + 1]);
+                        mx[2] = fmaxf(mx[2], s[i + 2]);
+                        mx[3] = fmaxf(mx[3], s[i + 3]);
+                    }
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+                    // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
+                    // P's type and the f32 sums carry without loss), so O is seldom rescaled.
+                    const bool grow = top > m + 8.f;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float mn = grow ? top : m, f = grow ? ex2(m - mn) : 1.f;  // m = -inf: the factor is 0
+                        m = mn;
+                        l *= f;
+                        if (st != sub) {
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i) {
+                                uint32_t o[16];
+                                tmem_ld16(tO + 16 * i, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                                tmem_st16(tO + 16 * i, o);
+                            }
+                        }
+                    }
+                    const float ms = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t u[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float p0 = ex2(fmaf(s[64 * i + 2 * j], a.scale_log2, -ms));
+                            const float p1 = ex2(fmaf(s[64 * i + 2 * j + 1], a.scale_log2, -ms));
+                            sum[(2 * j) & 3] += p0;
+                            sum[(2 * j + 1) & 3] += p1;
+                            u[j] = pack2<kHalf>(p0, p1);
+                        }
+                        tmem_st32(tP + 32 * i, u);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                mbar_arrive(&S.p_ready[wg]);
+            }
+            if (!ok) break;
+            if (!(ok = attn_wait(&S.o_full[wg], o_par, &S, a.status, 531))) break;
+            o_par ^= 1;
+            if (busy) {
+                tc_fence_after();
+                const int R = x.b < 0 ? kTile : a.suffix_rows;
+                const long long part = part_bytes(R, D);
+                unsigned char* dst = a.ws + (x.b < 0 ? a.ws_prefix : a.ws_suffix) + ((long long)(x.index + (int)blockIdx.x) * 2 + sub) * part;
+                const bool mine = rr < x.rows;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    float o[32];
+                    tmem_ld32(tO + 32 * i, o);
+                    tmem_ld_wait();
+                    if (mine) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            ((float4*)dst)[(8 * i + j) * R + row] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    }
+                }
+                if (mine) {
+                    float* ml = (float*)dst + (long long)R * D;
+                    ml[row] = m;
+                    ml[R + row] = l;
+                }
+                tc_fence_before();
+            }
+        }
+    } else if (warp == 8) {
+        // ---- tensor core ----
+        // The S product of a step is issued two steps ahead of its P V product: one cursor over the pieces makes S steps,
+        // their flags wait in a queue of two for the P V side.
+        constexpr uint32_t id_s = idesc_f16(kHalf, false, kTile), id_o = idesc_f16(kHalf, true, D);
+        unsigned ks = 0, vs = 0, qs = 0;  // running tile counts of the rings
+        uint32_t p_par[2] = {0, 0}, d_par[2] = {0, 0};
+        unsigned queue[2] = {0, 0};  // bit 0 accumulate, 1 last of the warpgroup, 2 releases V, 3 valid
+        unsigned n_s = 0, st = 0, ns = 0;
+        bool have = false, ok = true;
+        auto issue_s = [&]() -> bool {  // the next S step if there is one
+            queue[n_s & 1] = 0;
+            if (!have || st == ns) {
+                if (have) qs += x.pair() ? 2 : 1;
+                have = walk.next(x);
+                if (!have) return true;
+                st = 0;
+                ns = x.steps();
+            }
+            const bool pair = x.pair();
+            const int w = n_s & 1;
+            const unsigned q = qs + (pair ? st & 1 : 0), qi = q % C::kQ, ki = ks % C::kRing;
+            if (st < (pair ? 2u : 1u)) {
+                if (!attn_wait(&S.q_full[qi], (q / C::kQ) & 1, &S, a.status, 532)) return false;
+            }
+            if (!pair || !(st & 1)) {
+                if (!attn_wait(&S.k_full[ki], (ks / C::kRing) & 1, &S, a.status, 533)) return false;
+            }
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t qa = smem_u32(Qs + qi * C::kTileBytes), ka = smem_u32(Ks + ki * C::kTileBytes);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t o = (k >> 2) * (kTile * 128) + (k & 3) * 32;
+                    mma_ss(tmem + C::kS + w * 128, desc_sw128(qa + o), desc_sw128(ka + o), id_s, k > 0);
+                }
+                tc_commit(&S.s_full[w]);
+                if (!pair || (st & 1)) tc_commit(&S.k_empty[ki]);
+                if (st + (pair ? 2 : 1) >= ns) tc_commit(&S.q_empty[qi]);
+            }
+            __syncwarp();
+            queue[w] = (st >= 2 ? 1u : 0u) | (st + 2 >= ns ? 2u : 0u) | ((!pair || (st & 1)) ? 4u : 0u) | 8u;
+            if (!pair || (st & 1)) ++ks;
+            ++st;
+            ++n_s;
+            return true;
+        };
+        ok = issue_s() && issue_s();
+        for (unsigned n = 0; ok && n < n_s; ++n) {
+            const int w = n & 1;
+            const unsigned f = queue[w], vi = vs % C::kRing;
+            if (!(ok = attn_wait(&S.v_full[vi], (vs / C::kRing) & 1, &S, a.status, 534))) break;
+            if (!(ok = attn_wait(&S.p_ready[w], p_par[w], &S, a.status, 535))) break;
+            p_par[w] ^= 1;
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t va = smem_u32(Vs + vi * C::kTileBytes);
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                    mma_ts(tmem + C::kO + w * C::kOStep, tmem + C::kP + w * C::kPStep + 8 * k, desc_v(va + k * 2048), id_o, (f & 1u) | (k > 0));
+                if (C::kAlias) tc_commit(&S.pv_done[w]);
+                if (f & 4u) tc_commit(&S.v_empty[vi]);
+                if (f & 2u) tc_commit(&S.o_full[w]);
+            }
+            __syncwarp();
+            if (f & 4u) ++vs;
+            if (C::kAlias) {  // the next S of this warpgroup overwrites P
+                if (!(ok = attn_wait(&S.pv_done[w], d_par[w], &S, a.status, 536))) break;
+                d_par[w] ^= 1;
+            }
+            ok = issue_s();
+        }
+        // the tensor core has to be done before its memory is given back
+        if (lane == 0) tc_commit(&S.drain);
+        __syncwarp();
+        for (uint32_t i = 0; i < kWaitPolls && !mbar_try_wait(&S.drain, 0); ++i) {
+        }
+    } else if (warp == 9) {
+        // ---- K and V rows ----
+        bool ok = true;
+        while (ok && walk.next(x)) {
+            const int* trow = a.table + (long long)(x.b < 0 ? p.ref : x.b) * a.table_row;
+            const int stop = min(x.len, cap), kcol = x.h * a.k_head, vcol = x.h * a.v_head;
+            auto slots_of = [&](unsigned t, int (&y)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = x.key0 + (int)t * kTile + 4 * lane + i;
+                    y[i] = a.kv_rows;  // past the last row: the copy writes zeros, so nothing stale meets the products
+                    if (k < stop) {
+                        const int pg = a.page_shift >= 0 ? k >> a.page_shift : k / a.page;
+                        const long long slot = (long long)__ldg(trow + pg) * a.page + (k - pg * a.page);
+                        if (slot >= 0 && slot < a.kv_rows) y[i] = (int)slot;
+                        else batch_status(a.status, 4, 524, x.b, k);
+                    }
+                }
+            };
+            int y[4];
+            slots_of(x.t0, y);
+            for (unsigned t = x.t0; t < x.t1; ++t) {
+                const unsigned i = k_issued % C::kRing, par = ((k_issued / C::kRing) & 1) ^ 1;
+                if (!(ok = attn_wait(&S.k_empty[i], par, &S, a.status, 537))) break;
+                if (lane == 0) mbar_arrive_expect_tx(&S.k_full[i], C::kTileBytes);
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < C::kAtoms; ++c)
+                    gather4(Ks + i * C::kTileBytes + c * (kTile * 128) + lane * 512, &kmap, kcol + 64 * c, y[0], y[1], y[2], y[3], &S.k_full[i]);
+                ++k_issued;
+                int z[4] = {y[0], y[1], y[2], y[3]};
+                if (t + 1 < x.t1) slots_of(t + 1, y);
+                if (!(ok = attn_wait(&S.v_empty[i], par, &S, a.status, 538))) break;
+                if (lane == 0) mbar_arrive_expect_tx(&S.v_full[i], C::kTileBytes);
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < C::kAtoms; ++c)
+                    gather4(Vs + i * C::kTileBytes + c * (kTile * 128) + lane * 512, &vmap, vcol + 64 * c, z[0], z[1], z[2], z[3], &S.v_full[i]);
+                ++v_issued;
+            }
+        }
+    } else {
+        // ---- queries ----
+        const int t = tid - 320;  // 0 .. 63
+        unsigned q = 0;
+        bool ok = true;
+        while (ok && walk.next(x)) {
+            for (int half = 0; half < (x.pair() ? 2 : 1); ++half, ++q) {
+                const unsigned i = q % C::kQ;
+                if (!(ok = attn_wait(&S.q_empty[i], ((q / C::kQ) & 1) ^ 1, &S, a.status, 539))) break;
+                unsigned char* dst = Qs + i * C::kTileBytes;
+#pragma unroll 4
+                for (int j = t; j < kTile * (D / 8); j += 64) {
+                    const int r = j / (D / 8), c = j % (D / 8), rr = half * kTile + r, ir = x.rb * 2 * kTile + rr;
+                    const int tok = ir / a.G, head = x.h * a.G + ir - tok * a.G;
+                    const bool valid = rr < x.rows;
+                    const unsigned char* src =
+                        (const unsigned char*)a.q + (valid ? ((long long)(x.first + tok) * a.q_row + head * a.q_head + c * 8) * 2 : 0);
+                    cp_async16(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, valid);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_proxy_async_smem();
+                mbar_arrive(&S.q_full[i]);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (warp == 9 && *(volatile int*)&S.abort) {
+        // a role gave up: copies may still be on their way into this CTA's shared memory, so the last of each stage lands first
+        auto landed = [&](uint64_t* full, unsigned issued) {
+            for (unsigned i = 0; i < C::kRing; ++i) {
+                const unsigned n = issued > i ? (issued - i + C::kRing - 1) / C::kRing : 0;  // copies into stage i
+                for (uint32_t j = 0; n > 0 && j < kWaitPolls && !mbar_try_wait(full + i, (n - 1) & 1); ++j) {
+                }
+            }
+        };
+        landed(S.k_full, k_issued);
+        landed(S.v_full, v_issued);
+    }
+}
+
+// ---- merge --------------------------------------------------------------------------------------------------------------
+// Row r of an item's pieces: M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L. D / 4 lanes share a row (four
+// output columns each). Neighbouring rows are neighbouring heads of a token, so a warp's reads of a piece are contiguous
+// across its rows.
+template <int D, bool kHalf>
+__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixAttnArgs a) {
+    constexpr int L = D / 4, kRows = 256 / L;
+    griddep_wait();
+    const PlanHead h = *(const PlanHead*)a.ws;
+    const unsigned* cum = (const unsigned*)(a.ws + 256);
+    const long long id = (long long)blockIdx.x * kRows + threadIdx.x / L;
+    const int lane = threadIdx.x % L;
+    const int tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
+    if (tok >= (int)h.tokens) return;
+    const int b = request_of(a, tok);
+    const Req r = request(a, b, nullptr);
+    const int j = tok - r.first;
+    if (j < 0 || j >= r.n) return;
+    const int kv = head / a.G, hg = head - kv * a.G;
+
+    float M = -INFINITY, Ls = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float m, float l, const float4& v) {  // one more piece: m = -inf, l = 0 leaves everything as it is
+        const float mn = m > M ? m : M;
+        const float f = M == mn ? 1.f : ex2(M - mn), g = m == mn ? (l == 0.f ? 0.f : 1.f) : (l == 0.f ? 0.f : ex2(m - mn));
+        M = mn;
+        Ls = Ls * f + l * g;
+        o.x = o.x * f + v.x * g;
+        o.y = o.y * f + v.y * g;
+        o.z = o.z * f + v.z * g;
+        o.w = o.w * f + v.w * g;
+    };
+    // all pieces of the item whose first step is `first`, for its block row `rr`
+    auto item = [&](unsigned first, unsigned tiles, int rows, int index, int rr, const unsigned char* base, int R) {
+        const int sh = rows > kTile ? 1 : 0;
+        const unsigned len = tiles << sh;
+        const int c0 = cta_of(first, h.total, a.ctas), c1 = cta_of(first + len - 1, h.total, a.ctas);
+        const long long part = part_bytes(R, D);
+        const int row = rr & (kTile - 1), half = rr >> 7;
+        for (int c = c0; c <= c1; ++c) {
+            const unsigned lo = max(range_lo(h.total, c, a.ctas), first), hi = min(range_lo(h.total, c + 1, a.ctas), first + len);
+            if (hi <= lo) continue;
+            const unsigned t0 = (lo - first + sh) >> sh, t1 = (hi - first + sh) >> sh;
+            if (t1 <= t0) continue;
+            const unsigned char* slot = base + (long long)(index + c) * 2 * part;
+            const int n = sh ? 1 : min(t1 - t0, 2u);
+            for (int s = 0; s < n; ++s) {
+                const float* src = (const float*)(slot + (sh ? half : s) * part);
+                const float4 v = ((const float4*)src)[lane * R + row];
+                add(src[(long long)R * D + row], src[(long long)R * D + R + row], v);
+            }
+        }
+    };
+    if (h.tiles > 0) {
+        const int total = (int)h.tokens * a.G, gr = tok * a.G + hg, rb = gr / (2 * kTile), blocks = row_blocks(total);
+        item(kv * h.per_head + rb * 2 * h.tiles, h.tiles, min(2 * kTile, total - rb * 2 * kTile), kv * blocks + rb, gr - rb * 2 * kTile,
+             a.ws + a.ws_prefix, kTile);
+    }
+    const unsigned tiles = own_tiles(a, r, (int)h.prefix);
+    if (tiles > 0) {
+        const int total = r.n * a.G, gr = j * a.G + hg, rb = gr / (2 * kTile), blocks = row_blocks(total);
+        const unsigned per_head = tiles * steps_of_rows(total);
+        item(cum[b] + kv * per_head + rb * 2 * tiles, tiles, min(2 * kTile, total - rb * 2 * kTile), (int)cum[a.batch + b] + kv * blocks + rb,
+             gr - rb * 2 * kTile, a.ws + a.ws_suffix, a.suffix_rows);
+    }
+    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;  // a row that saw no key is zero
+    uint2 w;
+    w.x = pack2<kHalf>(o.x * inv, o.y * inv);
+    w.y = pack2<kHalf>(o.z * inv, o.w * inv);
+    *(uint2*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * 4) * 2) = w;
+    if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + log2f(Ls)) * kLn2;
+}
+
+template <int D, bool kHalf>
+static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s, bool pdl) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.ctas);
+    cfg.blockDim = dim3(kAttnThreads);
+    cfg.dynamicSmemBytes = Cfg<D>::kSmem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_attn_kernel<D, kHalf>, a, k, v);
+    if (e != cudaSuccess) return e;
+    constexpr int rows = 256 / (D / 4);
+    cfg.gridDim = dim3((unsigned)(((long long)a.rows * a.qh + rows - 1) / rows));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;  // its wait is its first statement, so it may always start under the first kernel's tail
+    return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf>, a);
+}
+
+cudaError_t prefix_attn_launch(const PrefixAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, int dim, bool fp16, cudaStream_t s, bool pdl) {
+    if (dim == 64) return fp16 ? prefix_attn_run<64, true>(a, k, v, s, pdl) : prefix_attn_run<64, false>(a, k, v, s, pdl);
+    return fp16 ? prefix_attn_run<128, true>(a, k, v, s, pdl) : prefix_attn_run<128, false>(a, k, v, s, pdl);
+}
+
+cudaError_t prefix_attn_prepare() {
+    cudaError_t e = cudaFuncSetAttribute(prefix_attn_kernel<64, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<64>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(prefix_attn_kernel<64, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<64>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(prefix_attn_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<128>::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(prefix_attn_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<128>::kSmem);
+    return e;
+}
+
+}  // namespace mk

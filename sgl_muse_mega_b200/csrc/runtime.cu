@@ -10,6 +10,7 @@
 #include <new>
 
 #include "../../include/mk_abi.h"
+#include "batch.h"
 #include "draft.h"
 #include "stages.h"
 
@@ -92,6 +93,14 @@ struct MkLaunch {
     mk::SoftcapArgs softcap;
     mk::AcceptArgs accept;
     mk::GemmArgs op_gemm;
+    // the batched step's cache path
+    mk::BlockTablesArgs tables;
+    mk::RopeTableArgs rope_table;
+    mk::RotaryArgs rotary;
+    mk::PrefixAttnArgs pattn;
+    CUtensorMap k_map, v_map;
+    int head_dim;
+    bool fp16, interleaved;
     // the DFlash2 draft's launch lists: n_dops > 0 replaces both of the above
     mk::DraftOp* dops;
     int n_dops;
@@ -100,7 +109,7 @@ struct MkLaunch {
 // the L2, 0.5 - 1 us: seconds)
 enum XchgPoint { XP_AR = 0, XP_POOL, XP_Z, XP_ZB, XP_UNPOOL, XP_LOGITS };
 static const long long kDefaultWaitBudget = 1ll << 22;
-enum OpKind { OP_FEEDS = 1, OP_ENTRY, OP_GEMM_BF16, OP_SOFTCAP, OP_ACCEPT };
+enum OpKind { OP_FEEDS = 1, OP_ENTRY, OP_GEMM_BF16, OP_SOFTCAP, OP_ACCEPT, OP_BLOCK_TABLES, OP_ROPE_TABLE, OP_ROTARY, OP_PREFIX_ATTN };
 
 using namespace mk;
 
@@ -211,6 +220,10 @@ int mk_module_load(const void* image, uint64_t bytes, const char* code_prefetch_
     if (e != cudaSuccess) return cuda_fail(e, "fused_prepare");
     e = draft_prepare();
     if (e != cudaSuccess) return cuda_fail(e, "draft_prepare");
+    e = batch_prepare();
+    if (e != cudaSuccess) return cuda_fail(e, "batch_prepare");
+    e = prefix_attn_prepare();
+    if (e != cudaSuccess) return cuda_fail(e, "prefix_attn_prepare");
     MkModule* m = new (std::nothrow) MkModule{dev, prop.multiProcessorCount};
     MK_REQUIRE(m != nullptr, "out of host memory");
     *out = m;
@@ -933,7 +946,23 @@ int mk_launch_step(const MkLaunch* launch, uint64_t stream, int64_t first, int64
     return 0;
 }
 
+// the launch's device for the length of a call
+struct OnDevice {
+    int before;
+    cudaError_t e;
+    explicit OnDevice(int device) : before(-1) {
+        e = cudaGetDevice(&before);
+        if (e != cudaSuccess || before == device) before = -1;
+        else e = cudaSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
 static int run_ops(const MkLaunch* L, cudaStream_t s, bool pdl) {
+    const OnDevice dev(L->device);
+    if (dev.e != cudaSuccess) return cuda_fail(dev.e, "cudaSetDevice");
     for (int i = 0; i < L->n_ops; ++i) {
         cudaError_t e = cudaSuccess;
         switch (L->op_kind[i]) {
@@ -942,6 +971,10 @@ static int run_ops(const MkLaunch* L, cudaStream_t s, bool pdl) {
             case OP_GEMM_BF16: e = gemm_launch(L->op_gemm, false, s, pdl); break;
             case OP_SOFTCAP: e = softcap_launch(L->softcap, s, pdl); break;
             case OP_ACCEPT: e = accept_launch(L->accept, s, pdl); break;
+            case OP_BLOCK_TABLES: e = block_tables_launch(L->tables, L->sms, s, pdl); break;
+            case OP_ROPE_TABLE: e = rope_table_launch(L->rope_table, L->sms, s, pdl); break;
+            case OP_ROTARY: e = rotary_launch(L->rotary, L->fp16, L->interleaved, s, pdl); break;
+            case OP_PREFIX_ATTN: e = prefix_attn_launch(L->pattn, L->k_map, L->v_map, L->head_dim, L->fp16, s, pdl); break;
             default: return fail("op %d does not exist", L->op_kind[i]);
         }
         if (e != cudaSuccess) return fail("op %d launch: %s", L->op_kind[i], cudaGetErrorString(e));
@@ -1048,6 +1081,10 @@ int mk_launch_info(const MkLaunch* launch, MkLaunchInfo* out) {
         out->cluster = 1;
         out->grid = L->op_kind[0] == OP_GEMM_BF16 ? gemm_grid(L->op_gemm) : 16;
         out->smem = L->op_kind[0] == OP_GEMM_BF16 ? (int64_t)gemm_smem(L->op_gemm, false) : 0;
+        if (L->op_kind[0] == OP_PREFIX_ATTN) {
+            out->kernels = 2;
+            out->grid = L->pattn.ctas;
+        }
         out->param_bytes = (int64_t)sizeof(MkLaunch);
         return 0;
     }
@@ -1461,3 +1498,4 @@ int mk_launch_status(const MkLaunch* launch, uint64_t stream, MkLaunchStatus* ou
 }  // extern "C"
 
 #include "draft_host.inc"
+#include "batch_host.inc"
