@@ -84,6 +84,8 @@ struct PrefixAttnArgs {
     const int* prefix_len;
     int batch, rows, max_new, qh, kvh, G, page, page_shift, kv_rows, window, suffix_rows;
     int k_head, v_head;  // elements between the heads of a cache row
+    int run;             // rows of a copy: the largest power of two up to 128 that divides the page
+    int q_box;           // the queries of a tile are 128 / G whole tokens: copied as a box
     float scale_log2;
     unsigned char* ws;
     long long ws_prefix, ws_suffix;  // byte offsets of the partials in ws
@@ -91,11 +93,15 @@ struct PrefixAttnArgs {
     int* status;
 };
 
+// tensor maps of 64-element wide columns: boxes of `run` cache rows, single cache rows (for gathers), G heads x 128 / G tokens
+struct PrefixAttnMaps {
+    CUtensorMap k_run, v_run, k_row, v_row, q;
+};
+
 cudaError_t block_tables_launch(const BlockTablesArgs& a, int sms, cudaStream_t s, bool pdl);
 cudaError_t rope_table_launch(const RopeTableArgs& a, int sms, cudaStream_t s, bool pdl);
 cudaError_t rotary_launch(const RotaryArgs& a, bool fp16, bool interleaved, cudaStream_t s, bool pdl);
-cudaError_t prefix_attn_launch(const PrefixAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, int dim, bool fp16, cudaStream_t s,
-                               bool pdl);
+cudaError_t prefix_attn_launch(const PrefixAttnArgs& a, const PrefixAttnMaps& maps, int dim, bool fp16, cudaStream_t s, bool pdl);
 size_t block_tables_smem(int batch, int pool_rows);
 cudaError_t batch_prepare();
 cudaError_t prefix_attn_prepare();

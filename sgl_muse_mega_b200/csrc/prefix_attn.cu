@@ -16,8 +16,8 @@
 // item or the next CTA, so the slots are distinct. prefix_merge_kernel adds the pieces of each row, in slot order.
 //
 // A CTA's twelve warps: two softmax warpgroups (a thread holds one query row, its scores are one TMEM lane), one thread
-// that issues the tensor-core products, a warp that gathers K and V rows (TMA gather of four cache rows a lane, so any
-// page size costs the same), two that gather the queries. Steps alternate between the two warpgroups, each with its own
+// that issues the tensor-core products, a warp each that brings in K rows, V rows (TMA boxes of a page's rows, or gathers of
+// four rows where pages are small or odd) and queries. Steps alternate between the two warpgroups, each with its own
 // S, P and O in tensor memory: while one takes the exponentials of its step the tensor core works for the other.
 #include "batch.h"
 #include "umma.cuh"
@@ -30,31 +30,32 @@ using namespace umma;
 constexpr int kTile = 128;  // rows of a step and keys of a tile
 constexpr int kAttnThreads = 384;
 constexpr float kLn2 = 0.69314718055994530942f;
+// What an item costs besides its steps (its queries in, its O out, the tensor core's start), counted in steps
+constexpr unsigned kItemSteps = 1;
 
 // ---- the plan: the same numbers in every warp of both kernels ---------------------------------------------------------
 struct PlanHead {  // in front of the scratch, for the merge kernel
-    unsigned total, prefix_steps, tiles, row_blocks, per_head, p_lo, prefix, tokens;
+    unsigned total, prefix_steps, tiles, pad, per_head, p_lo, prefix, tokens;
 };
 
 struct Req {
     int first, n, len;  // its first row, its rows, its keys
 };
 // the lengths of request b as far as they are usable: what contradicts the launch's extents is left out (and recorded)
-__device__ __forceinline__ Req request(const PrefixAttnArgs& a, int b, int* status) {
-    Req r;
-    r.first = __ldg(a.cu_rows + b);
-    r.n = __ldg(a.cu_rows + b + 1) - r.first;
-    r.len = __ldg(a.kv_lens + b);
-    const long long cap = (long long)a.width * a.page;
+__device__ __forceinline__ Req usable(const PrefixAttnArgs& a, int b, int c0, int c1, int len, int* status) {
+    Req r{c0, c1 - c0, len};
     if (r.n < 0 || r.n > a.max_new || r.first < 0 || r.first + r.n > a.rows) {
         if (status != nullptr) batch_status(status, 4, 520, b, r.n);
         r.n = 0;
     }
-    if (r.len < 0 || r.len > cap) {
+    if (r.len < 0 || r.len > a.width * a.page) {
         if (status != nullptr) batch_status(status, 4, 521, b, r.len);
         r.n = 0;
     }
     return r;
+}
+__device__ __forceinline__ Req request(const PrefixAttnArgs& a, int b) {
+    return usable(a, b, __ldg(a.cu_rows + b), __ldg(a.cu_rows + b + 1), __ldg(a.kv_lens + b), nullptr);
 }
 // steps of one key tile over all row blocks of `rows` rows: two for every 256 rows, one for a rest of up to 128
 __device__ __forceinline__ unsigned steps_of_rows(int rows) { return (unsigned)((rows + kTile - 1) / kTile); }
@@ -62,15 +63,27 @@ __device__ __forceinline__ int own_first(const PrefixAttnArgs& a, const Req& r, 
     const int lo = a.window > 0 ? max(0, r.len - r.n - a.window) : 0;
     return max(prefix, lo);
 }
+// where its tile 0 starts: the runs of cache rows that one copy brings in begin at multiples of their length
+__device__ __forceinline__ int own_start(const PrefixAttnArgs& a, const Req& r, int prefix) { return own_first(a, r, prefix) & ~(a.run - 1); }
 __device__ __forceinline__ unsigned own_tiles(const PrefixAttnArgs& a, const Req& r, int prefix) {
-    const int k0 = own_first(a, r, prefix);
-    return r.n > 0 && r.len > k0 ? (unsigned)(r.len - k0 + kTile - 1) / kTile : 0u;
-}
-__device__ __forceinline__ unsigned own_steps(const PrefixAttnArgs& a, const Req& r, int prefix) {
-    return own_tiles(a, r, prefix) * steps_of_rows(r.n * a.G) * a.kvh;
+    if (r.n <= 0 || r.len <= own_first(a, r, prefix)) return 0u;
+    return (unsigned)(r.len - own_start(a, r, prefix) + kTile - 1) / kTile;
 }
 __device__ __forceinline__ int row_blocks(int rows) { return (rows + 2 * kTile - 1) / (2 * kTile); }
+// steps of all row blocks of `rows` rows over `tiles` key tiles, for one kv head
+__device__ __forceinline__ unsigned head_steps(unsigned tiles, int rows) {
+    return tiles > 0 ? tiles * steps_of_rows(rows) + row_blocks(rows) * kItemSteps : 0u;
+}
+__device__ __forceinline__ unsigned own_steps(const PrefixAttnArgs& a, const Req& r, int prefix) {
+    return head_steps(own_tiles(a, r, prefix), r.n * a.G) * a.kvh;
+}
 __device__ __forceinline__ int own_items(const PrefixAttnArgs& a, const Req& r) { return row_blocks(r.n * a.G) * a.kvh; }
+// the key tiles of an item that the steps [lo, hi) of it stand for; a range that ends inside a pair of steps leaves the pair
+// to the range that starts it
+__device__ __forceinline__ void tiles_of(unsigned lo, unsigned hi, int sh, unsigned& t0, unsigned& t1) {
+    t0 = ((lo > kItemSteps ? lo - kItemSteps : 0u) + sh) >> sh;
+    t1 = ((hi > kItemSteps ? hi - kItemSteps : 0u) + sh) >> sh;
+}
 
 struct Plan {
     int prefix;         // shared keys (0: none shared)
@@ -82,50 +95,56 @@ struct Plan {
     unsigned prefix_steps, total;
 };
 
-// One warp; every lane gets the result. Three passes over the batch's lengths, which stay in L1.
+// One warp; every lane gets the result. Two passes over the batch's lengths; all loads that open the first are issued at
+// once, the second finds them in L1 (a lane's first request stays in registers).
 __device__ Plan make_plan(const PrefixAttnArgs& a, int lane, int* status, unsigned* cum) {
     Plan p;
-    const int cap = (int)min((long long)a.width * a.page, 0x7fffffffll);
+    const int cap = a.width * a.page;  // below 2^30 + page
+    const int at = min(lane, a.batch - 1);
     int want = __ldg(a.prefix_len);
+    p.tokens = __ldg(a.cu_rows + a.batch);
+    const int c0 = __ldg(a.cu_rows + at), c1 = __ldg(a.cu_rows + at + 1), len = __ldg(a.kv_lens + at);
     if (want < 0 || want > cap) {
         if (status != nullptr) batch_status(status, 4, 522, want, cap);
         want = 0;
     }
-    p.tokens = __ldg(a.cu_rows + a.batch);
     if (p.tokens < 0 || p.tokens > a.rows) {
         if (status != nullptr) batch_status(status, 4, 523, p.tokens, a.rows);
         p.tokens = 0;
     }
+    const Req mine = lane < a.batch ? usable(a, lane, c0, c1, len, status) : Req{0, 0, 0};
     int live = 0, ref = 0x7fffffff, lo = 0x7fffffff, hi = 0;
     for (int b = lane; b < a.batch; b += 32) {
-        const Req r = request(a, b, status);
+        const Req r = b == lane ? mine : usable(a, b, __ldg(a.cu_rows + b), __ldg(a.cu_rows + b + 1), __ldg(a.kv_lens + b), status);
         if (r.n <= 0 || r.len <= 0) continue;
         ++live;
         if (r.len >= want) ref = min(ref, b);
         lo = min(lo, a.window > 0 ? max(0, r.len - r.n - a.window) : 0);
         hi = max(hi, min(want, r.len));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        live += __shfl_xor_sync(0xffffffffu, live, o);
-        ref = min(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
+    live = __reduce_add_sync(0xffffffffu, live);
+    ref = __reduce_min_sync(0xffffffffu, ref);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
     // one request shares with nobody, and a prefix that no request holds whole cannot be read through one table row
     p.prefix = live > 1 && ref != 0x7fffffff ? want : 0;
     p.ref = p.prefix > 0 ? ref : 0;
     p.p_lo = p.prefix > 0 ? lo / kTile * kTile : 0;
     p.tiles = p.prefix > 0 && hi > p.p_lo ? (unsigned)(hi - p.p_lo + kTile - 1) / kTile : 0u;
-    p.per_head = p.tiles * steps_of_rows(p.tokens * a.G);
+    p.per_head = head_steps(p.tiles, p.tokens * a.G);
     p.prefix_steps = p.per_head * a.kvh;
     unsigned sum = p.prefix_steps;
     int items = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
         const int b = b0 + lane;
         Req r{0, 0, 0};
-        if (b < a.batch) r = request(a, b, nullptr);
+        if (b0 == 0) r = mine;
+        else if (b < a.batch) r = request(a, b);
         const unsigned x = own_steps(a, r, p.prefix);
+        if (cum == nullptr) {
+            sum += __reduce_add_sync(0xffffffffu, x);
+            continue;
+        }
         const int it = own_items(a, r);
         unsigned inc = x;
         int ci = it;
@@ -135,7 +154,7 @@ __device__ Plan make_plan(const PrefixAttnArgs& a, int lane, int* status, unsign
             const int z = __shfl_up_sync(0xffffffffu, ci, o);
             if (lane >= o) inc += y, ci += z;
         }
-        if (cum != nullptr && b < a.batch) {  // first step and first item of each request
+        if (b < a.batch) {  // first step and first item of each request, for the merge
             cum[b] = sum + inc - x;
             cum[a.batch + b] = (unsigned)(items + ci - it);
         }
@@ -146,8 +165,13 @@ __device__ Plan make_plan(const PrefixAttnArgs& a, int lane, int* status, unsign
     return p;
 }
 
-__device__ __forceinline__ unsigned range_lo(unsigned total, int c, int ctas) { return (unsigned)((unsigned long long)total * c / ctas); }
+// first step of CTA c's range: floor(total c / ctas), without a 64-bit division
+__device__ __forceinline__ unsigned range_lo(unsigned total, int c, int ctas) {
+    const unsigned n = (unsigned)ctas, q = total / n;
+    return q * c + (total - q * n) * c / n;
+}
 __device__ __forceinline__ int cta_of(unsigned step, unsigned total, int ctas) {  // whose range holds the step
+    if (total < (1u << 24)) return (int)(((step + 1) * (unsigned)ctas - 1) / total);  // ctas <= 148 < 2^8
     return (int)((((unsigned long long)step + 1) * ctas - 1) / total);
 }
 
@@ -169,27 +193,30 @@ struct Piece {
 struct Walker {
     const PrefixAttnArgs& a;
     const Plan& p;
-    unsigned pos, end;  // steps left: [pos, end)
-    int b;              // -1 while in the prefix
-    unsigned base;      // first step of the current request's items (or 0)
-    int items;          // own items before request b
+    unsigned left;  // steps left
+    int b;          // -1 while in the prefix
+    int items;      // own items before request b
+    int h, rb;      // the next item
+    unsigned off;   // steps of it that lie before the range
     Req r;
-    unsigned tiles, per_head;
-    int row_total;
+    unsigned tiles;
+    int row_total, blocks, key0;
 
     __device__ Walker(const PrefixAttnArgs& a_, const Plan& p_, int cta, int lane) : a(a_), p(p_) {
-        pos = range_lo(p.total, cta, a.ctas);
-        end = range_lo(p.total, cta + 1, a.ctas);
+        unsigned pos = range_lo(p.total, cta, a.ctas);
+        left = range_lo(p.total, cta + 1, a.ctas) - pos;
         b = -1;
-        base = 0;
         items = 0;
-        if (pos >= p.prefix_steps && pos < end) {  // starts in a request's items: find it, the whole warp together
+        h = rb = 0;
+        off = 0;
+        blocks = 0;
+        if (left == 0) return;
+        if (pos >= p.prefix_steps) {  // starts in a request's items: find it, the whole warp together
             unsigned sum = p.prefix_steps;
-            int cnt = 0;
             for (int b0 = 0; b0 < a.batch; b0 += 32) {
                 const int bb = b0 + lane;
                 Req q{0, 0, 0};
-                if (bb < a.batch) q = request(a, bb, nullptr);
+                if (bb < a.batch) q = request(a, bb);
                 const unsigned x = own_steps(a, q, p.prefix);
                 const int it = own_items(a, q);
                 unsigned inc = x;
@@ -204,67 +231,58 @@ struct Walker {
                 if (hit != 0u) {
                     const int l = __ffs(hit) - 1;
                     b = b0 + l;
-                    base = sum + __shfl_sync(0xffffffffu, inc - x, l);
-                    items = cnt + __shfl_sync(0xffffffffu, ci - it, l);
+                    pos -= sum + __shfl_sync(0xffffffffu, inc - x, l);
+                    items += __shfl_sync(0xffffffffu, ci - it, l);
                     break;
                 }
                 sum += __shfl_sync(0xffffffffu, inc, 31);
-                cnt += __shfl_sync(0xffffffffu, ci, 31);
+                items += __shfl_sync(0xffffffffu, ci, 31);
             }
-            load();
         }
+        load();
+        const unsigned per_head = head_steps(tiles, row_total), block = 2 * tiles + kItemSteps;
+        h = (int)(pos / per_head);
+        pos -= h * per_head;
+        rb = (int)(pos / block);
+        off = pos - rb * block;
     }
     __device__ __forceinline__ void load() {
-        r = request(a, b, nullptr);
-        tiles = own_tiles(a, r, p.prefix);
+        if (b < 0) {
+            tiles = p.tiles;
+            r = Req{0, p.tokens, p.prefix};
+            key0 = p.p_lo;
+        } else {
+            r = request(a, b);
+            tiles = own_tiles(a, r, p.prefix);
+            key0 = own_start(a, r, p.prefix);
+        }
         row_total = r.n * a.G;
-        per_head = tiles * steps_of_rows(row_total);
+        blocks = row_blocks(row_total);
     }
     // the next piece, false at the end of the range
     __device__ bool next(Piece& x) {
-        while (pos < end) {
-            unsigned off;
-            if (pos < p.prefix_steps) {
-                x.b = -1;
-                row_total = p.tokens * a.G;
-                tiles = p.tiles;
-                per_head = p.per_head;
-                off = pos;
-                x.first = 0;
-                x.n = p.tokens;
-                x.len = p.prefix;
-                x.key0 = p.p_lo;
-            } else {
-                if (b < 0) {  // out of the prefix
-                    b = 0;
-                    base = p.prefix_steps;
-                    load();
-                }
-                while (pos >= base + per_head * a.kvh) {
-                    base += per_head * a.kvh;
-                    items += row_blocks(row_total) * a.kvh;
-                    ++b;
-                    load();
-                }
-                x.b = b;
-                off = pos - base;
-                x.first = r.first;
-                x.n = r.n;
-                x.len = r.len;
-                x.key0 = own_first(a, r, p.prefix);
+        while (left > 0) {
+            while (tiles == 0 || h == a.kvh) {  // on to the next request that has steps
+                if (b >= 0) items += blocks * a.kvh;
+                ++b;
+                h = 0;
+                load();
             }
-            x.h = (int)(off / per_head);
-            off -= x.h * per_head;
-            x.rb = (int)(off / (2 * tiles));
-            off -= x.rb * 2 * tiles;
-            const int blocks = row_blocks(row_total);
-            x.rows = min(2 * kTile, row_total - x.rb * 2 * kTile);
-            x.index = (x.b < 0 ? 0 : items) + x.h * blocks + x.rb;
+            x.b = b;
+            x.h = h;
+            x.rb = rb;
+            x.rows = min(2 * kTile, row_total - rb * 2 * kTile);
+            x.first = r.first;
+            x.n = r.n;
+            x.len = r.len;
+            x.key0 = key0;
+            x.index = (b < 0 ? 0 : items) + h * blocks + rb;
             const int sh = x.rows > kTile ? 1 : 0;
-            const unsigned len = tiles << sh, stop = min(off + (end - pos), len);
-            x.t0 = (off + sh) >> sh;  // a range that ends inside a pair of steps leaves the pair to the range that starts it
-            x.t1 = (stop + sh) >> sh;
-            pos += stop - off;
+            const unsigned len = (tiles << sh) + kItemSteps, stop = min(off + left, len);
+            tiles_of(off, stop, sh, x.t0, x.t1);
+            left -= stop - off;
+            off = 0;
+            if (++rb == blocks) rb = 0, ++h;
             if (x.t1 > x.t0) return true;
         }
         return false;
@@ -291,7 +309,7 @@ struct Cfg {
 
 struct Bars {
     uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[4], q_empty[4];
-    uint64_t s_full[2], p_ready[2], o_full[2], pv_done[2];
+    uint64_t s_full[2], s_free[2], p_ready[2], o_full[2], pv_done[2];
     uint64_t drain;
     uint32_t tmem;
     int abort;
@@ -303,6 +321,22 @@ __device__ __forceinline__ void gather4(void* dst, const CUtensorMap* map, int x
             smem_u32(dst)),
         "l"(map), "r"(x), "r"(y0), "r"(y1), "r"(y2), "r"(y3), "r"(smem_u32(bar))
         : "memory");
+}
+
+__device__ __forceinline__ void load_box2(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void load_box3(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 // D[128 x N] (+)= A B^T, both operands in shared memory
@@ -346,19 +380,26 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, float* r) {
           "=r"(u[31])
         : "r"(t));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t* u) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
-        "%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
-        "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]),
-        "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]),
-        "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
-        : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two f32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+    return r;
 }
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -394,21 +435,21 @@ __device__ __forceinline__ void row_keys(const PrefixAttnArgs& a, const Plan& p,
     int n = x.n, len = x.len, idx = j;
     if (x.b < 0) {
         const int b = request_of(a, j);
-        const Req r = request(a, b, nullptr);
+        const Req r = request(a, b);
         n = r.n;
         len = r.len;
         idx = j - r.first;
         if (idx >= n) return;  // a request that was left out
     }
     const int at = len - n + idx;  // its position
-    lo = a.window > 0 ? max(0, at - a.window) : 0;
+    lo = max(x.b < 0 ? 0 : p.prefix, a.window > 0 ? at - a.window : 0);
     hi = min(at + 1, x.b < 0 ? p.prefix : len);
     if (hi < lo) hi = lo;
 }
 
 template <int D, bool kHalf>
 __global__ void __launch_bounds__(kAttnThreads, 1)
-    prefix_attn_kernel(const PrefixAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    prefix_attn_kernel(const PrefixAttnArgs a, const __grid_constant__ PrefixAttnMaps maps) {
     typedef Cfg<D> C;
     extern __shared__ unsigned char raw[];
     __shared__ Bars S;
@@ -423,12 +464,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             mbar_init(&S.k_empty[i], 1);
             mbar_init(&S.v_full[i], 1);
             mbar_init(&S.v_empty[i], 1);
-            mbar_init(&S.q_full[i], 64);
+            mbar_init(&S.q_full[i], a.q_box ? 1 : 32);
             mbar_init(&S.q_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&S.s_full[i], 1);
-            mbar_init(&S.p_ready[i], 128);
+            mbar_init(&S.s_free[i], 4);
+            mbar_init(&S.p_ready[i], 4);
             mbar_init(&S.o_full[i], 1);
             mbar_init(&S.pv_done[i], 1);
         }
@@ -447,20 +489,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const bool writer = blockIdx.x == 0 && warp == 0;
     const Plan p = make_plan(a, lane, writer ? a.status : nullptr, writer ? cum : nullptr);
     if (writer && lane == 0)
-        *(PlanHead*)a.ws = PlanHead{p.total, p.prefix_steps, p.tiles, steps_of_rows(p.tokens * a.G), p.per_head, (unsigned)p.p_lo, (unsigned)p.prefix,
+        *(PlanHead*)a.ws = PlanHead{p.total, p.prefix_steps, p.tiles, 0u, p.per_head, (unsigned)p.p_lo, (unsigned)p.prefix,
                                     (unsigned)p.tokens};
     Walker walk(a, p, blockIdx.x, lane);
     Piece x;
     const int cap = a.width * a.page;
-    unsigned k_issued = 0, v_issued = 0;  // warp 9: tiles requested
+    unsigned issued = 0, q_boxes = 0;  // tiles that this warp's copies were asked for
 
     if (warp < 8) {
         // ---- softmax ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int wg = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes in bits 16 ..
         const uint32_t tS = tmem + lanes + C::kS + wg * 128, tP = tmem + lanes + C::kP + wg * C::kPStep, tO = tmem + lanes + C::kO + wg * C::kOStep;
         unsigned g = 0;  // steps of earlier pieces
-        uint32_t s_par = 0, o_par = 0;
+        uint32_t s_par = 0, o_par = 0, pv_par = 1;  // pv: the wait for the step before the first returns at once
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
         bool ok = true;
         while (ok && walk.next(x)) {
             const unsigned ns = x.steps(), sub = (wg - g) & 1;
@@ -476,12 +520,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 const int kb = x.key0 + (int)(x.t0 + (pair ? st >> 1 : st)) * kTile;
                 if (!(ok = attn_wait(&S.s_full[wg], s_par, &S, a.status, 530))) break;
                 s_par ^= 1;
+                tc_fence_after();
+                float s[128];
                 if (busy) {
-                    tc_fence_after();
-                    float s[128];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) tmem_ld32(tS + 32 * i, s + 32 * i);
                     tmem_ld_wait();
+                }
+                if (!C::kAlias) {  // the scores are in registers: the tensor core may write the next ones
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&S.s_free[wg]);
+                }
+                if (busy) {
                     if (!__all_sync(0xffffffffu, (lo <= kb && hi >= kb + kTile) || rr >= x.rows)) {
                         const int c0 = lo - kb, c1 = hi - kb;
 #pragma unroll
@@ -489,52 +540,55 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 128; i += 4) {
-                        mx[0] = fmaxf(mx[0], s[i]);
-                        mx[1] = fmaxf(mx[1], s[i + 1]);
-                        mx[2] = fmaxf(mx[2], s[i + 2]);
-                        mx[3] = fmaxf(mx[3], s[i + 3]);
+                    for (int i = 0; i < 128; i += 8) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], fmaxf(s[i + j], s[i + 4 + j]));
                     }
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
                     // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
                     // P's type and the f32 sums carry without loss), so O is seldom rescaled.
                     const bool grow = top > m + 8.f;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float mn = grow ? top : m, f = grow ? ex2(m - mn) : 1.f;  // m = -inf: the factor is 0
-                        m = mn;
-                        l *= f;
-                        if (st != sub) {
+                    const bool any = __any_sync(0xffffffffu, grow);
+                    const float mn = grow ? top : m, f = grow ? ex2(m - mn) : 1.f;  // m = -inf: the factor is 0
+                    m = mn;
+                    l *= f;
+                    // the P V product of this warpgroup's last step has read P and updated O
+                    if (!C::kAlias && !(ok = attn_wait(&S.pv_done[wg], pv_par, &S, a.status, 540))) break;
+                    if (any && st != sub) {
+                        tc_fence_after();
 #pragma unroll
-                            for (int i = 0; i < D / 16; ++i) {
-                                uint32_t o[16];
-                                tmem_ld16(tO + 16 * i, o);
-                                tmem_ld_wait();
+                        for (int i = 0; i < D / 16; ++i) {
+                            uint32_t o[16];
+                            tmem_ld16(tO + 16 * i, o);
+                            tmem_ld_wait();
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                                tmem_st16(tO + 16 * i, o);
-                            }
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_st16(tO + 16 * i, o);
                         }
                     }
                     const float ms = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float2 neg = make_float2(-ms, -ms);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint32_t u[32];
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t u[16];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const float p0 = ex2(fmaf(s[64 * i + 2 * j], a.scale_log2, -ms));
-                            const float p1 = ex2(fmaf(s[64 * i + 2 * j + 1], a.scale_log2, -ms));
-                            sum[(2 * j) & 3] += p0;
-                            sum[(2 * j + 1) & 3] += p1;
-                            u[j] = pack2<kHalf>(p0, p1);
+                        for (int j = 0; j < 16; ++j) {
+                            float2 e = fma2(make_float2(s[32 * i + 2 * j], s[32 * i + 2 * j + 1]), scale2, neg);
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                            sum[j & 1] = add2(sum[j & 1], e);
+                            u[j] = pack2<kHalf>(e.x, e.y);
                         }
-                        tmem_st32(tP + 32 * i, u);
+                        tmem_st16(tP + 16 * i, u);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     tmem_st_wait();
                     tc_fence_before();
-                }
-                mbar_arrive(&S.p_ready[wg]);
+                } else if (!C::kAlias && !(ok = attn_wait(&S.pv_done[wg], pv_par, &S, a.status, 540))) break;
+                pv_par ^= 1;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.p_ready[wg]);
             }
             if (!ok) break;
             if (!(ok = attn_wait(&S.o_full[wg], o_par, &S, a.status, 531))) break;
@@ -566,16 +620,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
     } else if (warp == 8) {
         // ---- tensor core ----
-        // The S product of a step is issued two steps ahead of its P V product: one cursor over the pieces makes S steps,
-        // their flags wait in a queue of two for the P V side.
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // The S product of step n + 2 comes before the P V product of step n where P has columns of its own (it waits for the
+        // scores of step n to have left S), behind it and after its end where P lies over S. One cursor over the pieces makes S
+        // steps, their flags wait in a queue of two for the P V side.
         constexpr uint32_t id_s = idesc_f16(kHalf, false, kTile), id_o = idesc_f16(kHalf, true, D);
         unsigned ks = 0, vs = 0, qs = 0;  // running tile counts of the rings
-        uint32_t p_par[2] = {0, 0}, d_par[2] = {0, 0};
-        unsigned queue[2] = {0, 0};  // bit 0 accumulate, 1 last of the warpgroup, 2 releases V, 3 valid
+        unsigned queue0 = 0, queue1 = 0;  // bit 0 accumulate, 1 last of the warpgroup, 2 releases V
         unsigned n_s = 0, st = 0, ns = 0;
         bool have = false, ok = true;
+        // what the issuing thread hands to the tensor core is made uniform over the warp first (shuffles from lane 0): the
+        // compiler then keeps descriptors in uniform registers
+        const uint64_t q_desc = desc_sw128(smem_u32(Qs)), k_desc = desc_sw128(smem_u32(Ks)), v_desc = desc_v(smem_u32(Vs));
         auto issue_s = [&]() -> bool {  // the next S step if there is one
-            queue[n_s & 1] = 0;
             if (!have || st == ns) {
                 if (have) qs += x.pair() ? 2 : 1;
                 have = walk.next(x);
@@ -584,8 +641,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 ns = x.steps();
             }
             const bool pair = x.pair();
-            const int w = n_s & 1;
-            const unsigned q = qs + (pair ? st & 1 : 0), qi = q % C::kQ, ki = ks % C::kRing;
+            const unsigned q = qs + (pair ? st & 1 : 0);
+            const int qi = __shfl_sync(0xffffffffu, (int)(q % C::kQ), 0), ki = __shfl_sync(0xffffffffu, (int)(ks % C::kRing), 0);
+            const int w = __shfl_sync(0xffffffffu, (int)(n_s & 1), 0);
+            const unsigned f = __shfl_sync(0xffffffffu, (st >= 2 ? 1u : 0u) | (st + 2 >= ns ? 2u : 0u) | ((!pair || (st & 1)) ? 4u : 0u) |
+                                                            (st + (pair ? 2 : 1) >= ns ? 8u : 0u), 0);
             if (st < (pair ? 2u : 1u)) {
                 if (!attn_wait(&S.q_full[qi], (q / C::kQ) & 1, &S, a.status, 532)) return false;
             }
@@ -593,98 +653,128 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 if (!attn_wait(&S.k_full[ki], (ks / C::kRing) & 1, &S, a.status, 533)) return false;
             }
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t qa = smem_u32(Qs + qi * C::kTileBytes), ka = smem_u32(Ks + ki * C::kTileBytes);
+            if (elect_one()) {
+                const uint64_t qd = q_desc + (uint64_t)(qi * (C::kTileBytes >> 4)), kd = k_desc + (uint64_t)(ki * (C::kTileBytes >> 4));
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t o = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-                    mma_ss(tmem + C::kS + w * 128, desc_sw128(qa + o), desc_sw128(ka + o), id_s, k > 0);
+                    const uint64_t o = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+                    mma_ss(tmem + C::kS + w * 128, qd + o, kd + o, id_s, k > 0);
                 }
                 tc_commit(&S.s_full[w]);
-                if (!pair || (st & 1)) tc_commit(&S.k_empty[ki]);
-                if (st + (pair ? 2 : 1) >= ns) tc_commit(&S.q_empty[qi]);
+                if (f & 4u) tc_commit(&S.k_empty[ki]);
+                if (f & 8u) tc_commit(&S.q_empty[qi]);
             }
             __syncwarp();
-            queue[w] = (st >= 2 ? 1u : 0u) | (st + 2 >= ns ? 2u : 0u) | ((!pair || (st & 1)) ? 4u : 0u) | 8u;
-            if (!pair || (st & 1)) ++ks;
+            if (w) queue1 = f;
+            else queue0 = f;
+            if (f & 4u) ++ks;
             ++st;
             ++n_s;
             return true;
         };
         ok = issue_s() && issue_s();
         for (unsigned n = 0; ok && n < n_s; ++n) {
-            const int w = n & 1;
-            const unsigned f = queue[w], vi = vs % C::kRing;
+            const int w = __shfl_sync(0xffffffffu, (int)(n & 1), 0);
+            const uint32_t par = (n >> 1) & 1;  // every warpgroup barrier completes once a step
+            const unsigned f = __shfl_sync(0xffffffffu, w ? queue1 : queue0, 0);
+            const int vi = __shfl_sync(0xffffffffu, (int)(vs % C::kRing), 0);
+            if (!C::kAlias) {
+                if (!(ok = attn_wait(&S.s_free[w], par, &S, a.status, 536))) break;
+                if (!(ok = issue_s())) break;
+            }
             if (!(ok = attn_wait(&S.v_full[vi], (vs / C::kRing) & 1, &S, a.status, 534))) break;
-            if (!(ok = attn_wait(&S.p_ready[w], p_par[w], &S, a.status, 535))) break;
-            p_par[w] ^= 1;
+            if (!(ok = attn_wait(&S.p_ready[w], par, &S, a.status, 535))) break;
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t va = smem_u32(Vs + vi * C::kTileBytes);
+            if (elect_one()) {
+                const uint64_t vd = v_desc + (uint64_t)(vi * (C::kTileBytes >> 4));
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
-                    mma_ts(tmem + C::kO + w * C::kOStep, tmem + C::kP + w * C::kPStep + 8 * k, desc_v(va + k * 2048), id_o, (f & 1u) | (k > 0));
-                if (C::kAlias) tc_commit(&S.pv_done[w]);
+                    mma_ts(tmem + C::kO + w * C::kOStep, tmem + C::kP + w * C::kPStep + 8 * k, vd + (uint64_t)(k * 2048 >> 4), id_o, k > 0 ? 1u : f & 1u);
+                tc_commit(&S.pv_done[w]);
                 if (f & 4u) tc_commit(&S.v_empty[vi]);
                 if (f & 2u) tc_commit(&S.o_full[w]);
             }
             __syncwarp();
             if (f & 4u) ++vs;
-            if (C::kAlias) {  // the next S of this warpgroup overwrites P
-                if (!(ok = attn_wait(&S.pv_done[w], d_par[w], &S, a.status, 536))) break;
-                d_par[w] ^= 1;
+            if (C::kAlias) {
+                if (!(ok = attn_wait(&S.pv_done[w], par, &S, a.status, 536))) break;
+                ok = issue_s();
             }
-            ok = issue_s();
         }
         // the tensor core has to be done before its memory is given back
-        if (lane == 0) tc_commit(&S.drain);
+        if (elect_one()) tc_commit(&S.drain);
         __syncwarp();
         for (uint32_t i = 0; i < kWaitPolls && !mbar_try_wait(&S.drain, 0); ++i) {
         }
-    } else if (warp == 9) {
-        // ---- K and V rows ----
+    } else if (warp == 9 || warp == 10) {
+        // ---- K rows (warp 9), V rows (warp 10) ----
+        // Where pages hold runs of 8 or more aligned rows, a lane copies a run as one box; else a lane gathers four rows. Rows
+        // past the piece's last key are asked for behind the pool's end, which reads zeros: a probability of zero times
+        // whatever a stale row holds would not be zero. So the run that the last key ends in is gathered row by row (V).
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        const bool is_v = warp == 10;
+        const CUtensorMap *run_map = is_v ? &maps.v_run : &maps.k_run, *row_map = is_v ? &maps.v_row : &maps.k_row;
+        unsigned char* ring = is_v ? Vs : Ks;
+        uint64_t *full = is_v ? S.v_full : S.k_full, *empty = is_v ? S.v_empty : S.k_empty;
+        const int head = is_v ? a.v_head : a.k_head;
+        const bool runs = a.run >= 8;
+        const int per = runs ? a.run : 4, mine = lane * per;  // this lane's keys of a tile
         bool ok = true;
         while (ok && walk.next(x)) {
             const int* trow = a.table + (long long)(x.b < 0 ? p.ref : x.b) * a.table_row;
-            const int stop = min(x.len, cap), kcol = x.h * a.k_head, vcol = x.h * a.v_head;
+            const int stop = min(x.len, cap), col = x.h * head;
+            auto slot_of = [&](int k, int n) -> int {  // pool row of key k, of n rows that lie in one page
+                if (k >= stop) return a.kv_rows;
+                const int pg = a.page_shift >= 0 ? k >> a.page_shift : k / a.page;
+                const long long slot = (long long)__ldg(trow + pg) * a.page + (k - pg * a.page);
+                if (slot >= 0 && slot + n <= a.kv_rows) return (int)slot;
+                batch_status(a.status, 4, 524, x.b, k);
+                return a.kv_rows;
+            };
             auto slots_of = [&](unsigned t, int (&y)[4]) {
+                const int k = x.key0 + (int)t * kTile + mine;
+                if (runs) {
+                    if (mine < kTile) y[0] = slot_of(k, min(per, stop - k));
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = x.key0 + (int)t * kTile + 4 * lane + i;
-                    y[i] = a.kv_rows;  // past the last row: the copy writes zeros, so nothing stale meets the products
-                    if (k < stop) {
-                        const int pg = a.page_shift >= 0 ? k >> a.page_shift : k / a.page;
-                        const long long slot = (long long)__ldg(trow + pg) * a.page + (k - pg * a.page);
-                        if (slot >= 0 && slot < a.kv_rows) y[i] = (int)slot;
-                        else batch_status(a.status, 4, 524, x.b, k);
-                    }
+                    for (int i = 0; i < 4; ++i) y[i] = slot_of(k + i, 1);
                 }
             };
-            int y[4];
+            int y[4] = {0, 0, 0, 0};
             slots_of(x.t0, y);
             for (unsigned t = x.t0; t < x.t1; ++t) {
-                const unsigned i = k_issued % C::kRing, par = ((k_issued / C::kRing) & 1) ^ 1;
-                if (!(ok = attn_wait(&S.k_empty[i], par, &S, a.status, 537))) break;
-                if (lane == 0) mbar_arrive_expect_tx(&S.k_full[i], C::kTileBytes);
+                const unsigned i = issued % C::kRing;
+                if (!(ok = attn_wait(&empty[i], ((issued / C::kRing) & 1) ^ 1, &S, a.status, 537))) break;
+                if (lane == 0) mbar_arrive_expect_tx(&full[i], C::kTileBytes);
                 __syncwarp();
+                unsigned char* dst = ring + i * C::kTileBytes + mine * 128;
+                if (mine < kTile) {
+                    const int k = x.key0 + (int)t * kTile + mine;
+                    if (!runs) {
 #pragma unroll
-                for (int c = 0; c < C::kAtoms; ++c)
-                    gather4(Ks + i * C::kTileBytes + c * (kTile * 128) + lane * 512, &kmap, kcol + 64 * c, y[0], y[1], y[2], y[3], &S.k_full[i]);
-                ++k_issued;
-                int z[4] = {y[0], y[1], y[2], y[3]};
+                        for (int c = 0; c < C::kAtoms; ++c)
+                            gather4(dst + c * (kTile * 128), row_map, col + 64 * c, y[0], y[1], y[2], y[3], &full[i]);
+                    } else if (is_v && k < stop && k + per > stop) {
+                        for (int j = 0; j < per; j += 4) {
+                            int z[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[e] = y[0] < a.kv_rows && k + j + e < stop ? y[0] + j + e : a.kv_rows;
+#pragma unroll
+                            for (int c = 0; c < C::kAtoms; ++c)
+                                gather4(dst + c * (kTile * 128) + j * 128, row_map, col + 64 * c, z[0], z[1], z[2], z[3], &full[i]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < C::kAtoms; ++c) load_box2(dst + c * (kTile * 128), run_map, col + 64 * c, y[0], &full[i]);
+                    }
+                }
+                ++issued;
                 if (t + 1 < x.t1) slots_of(t + 1, y);
-                if (!(ok = attn_wait(&S.v_empty[i], par, &S, a.status, 538))) break;
-                if (lane == 0) mbar_arrive_expect_tx(&S.v_full[i], C::kTileBytes);
-                __syncwarp();
-#pragma unroll
-                for (int c = 0; c < C::kAtoms; ++c)
-                    gather4(Vs + i * C::kTileBytes + c * (kTile * 128) + lane * 512, &vmap, vcol + 64 * c, z[0], z[1], z[2], z[3], &S.v_full[i]);
-                ++v_issued;
             }
         }
     } else {
         // ---- queries ----
-        const int t = tid - 320;  // 0 .. 63
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         unsigned q = 0;
         bool ok = true;
         while (ok && walk.next(x)) {
@@ -692,19 +782,32 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 const unsigned i = q % C::kQ;
                 if (!(ok = attn_wait(&S.q_empty[i], ((q / C::kQ) & 1) ^ 1, &S, a.status, 539))) break;
                 unsigned char* dst = Qs + i * C::kTileBytes;
-#pragma unroll 4
-                for (int j = t; j < kTile * (D / 8); j += 64) {
-                    const int r = j / (D / 8), c = j % (D / 8), rr = half * kTile + r, ir = x.rb * 2 * kTile + rr;
-                    const int tok = ir / a.G, head = x.h * a.G + ir - tok * a.G;
-                    const bool valid = rr < x.rows;
-                    const unsigned char* src =
-                        (const unsigned char*)a.q + (valid ? ((long long)(x.first + tok) * a.q_row + head * a.q_head + c * 8) * 2 : 0);
-                    cp_async16(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, valid);
+                const int ir = x.rb * 2 * kTile + half * kTile;  // the tile's first row in the item
+                if (a.q_box) {  // 128 / G whole tokens: one box a 64-wide column block
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&S.q_full[i], C::kTileBytes);
+#pragma unroll
+                        for (int c = 0; c < C::kAtoms; ++c)
+                            load_box3(dst + c * (kTile * 128), &maps.q, 64 * c, x.h * a.G, x.first + ir / a.G, &S.q_full[i]);
+                    }
+                    __syncwarp();
+                    ++q_boxes;
+                } else {
+#pragma unroll 1
+                    for (int r = lane; r < kTile; r += 32) {
+                        const bool valid = half * kTile + r < x.rows;
+                        const int tok = (ir + r) / a.G, head = x.h * a.G + ir + r - tok * a.G;
+                        const unsigned char* src =
+                            (const unsigned char*)a.q + (valid ? ((long long)(x.first + tok) * a.q_row + head * a.q_head) * 2 : 0);
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c)
+                            cp_async16(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + c * 16, valid);
+                    }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    fence_proxy_async_smem();
+                    mbar_arrive(&S.q_full[i]);
                 }
-                cp_async_commit();
-                cp_async_wait<0>();
-                fence_proxy_async_smem();
-                mbar_arrive(&S.q_full[i]);
             }
         }
     }
@@ -714,95 +817,131 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (warp == 9 && *(volatile int*)&S.abort) {
+    if (warp >= 9 && *(volatile int*)&S.abort) {
         // a role gave up: copies may still be on their way into this CTA's shared memory, so the last of each stage lands first
-        auto landed = [&](uint64_t* full, unsigned issued) {
-            for (unsigned i = 0; i < C::kRing; ++i) {
-                const unsigned n = issued > i ? (issued - i + C::kRing - 1) / C::kRing : 0;  // copies into stage i
+        auto landed = [&](uint64_t* full, unsigned stages, unsigned count) {
+            for (unsigned i = 0; i < stages; ++i) {
+                const unsigned n = count > i ? (count - i + stages - 1) / stages : 0;  // copies into stage i
                 for (uint32_t j = 0; n > 0 && j < kWaitPolls && !mbar_try_wait(full + i, (n - 1) & 1); ++j) {
                 }
             }
         };
-        landed(S.k_full, k_issued);
-        landed(S.v_full, v_issued);
+        if (warp == 11) landed(S.q_full, C::kQ, q_boxes);
+        else landed(warp == 10 ? S.v_full : S.k_full, C::kRing, issued);
     }
 }
 
+template <int N>
+struct Cols;
+template <>
+struct Cols<2> {
+    typedef float2 type;
+};
+template <>
+struct Cols<4> {
+    typedef float4 type;
+};
+
 // ---- merge --------------------------------------------------------------------------------------------------------------
-// Row r of an item's pieces: M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L. D / 4 lanes share a row (four
-// output columns each). Neighbouring rows are neighbouring heads of a token, so a warp's reads of a piece are contiguous
-// across its rows.
+// Row r of an item's pieces: M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L. A warp takes one row: its lanes
+// look up a piece each (the CTA's range, its slot, m and l; all loads of 32 pieces at once), then walk the pieces
+// together, D / 32 output columns a lane. The eight rows of a block are neighbours (heads of one token mostly), whose O
+// values share 128-byte lines.
 template <int D, bool kHalf>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixAttnArgs a) {
-    constexpr int L = D / 4, kRows = 256 / L;
+    constexpr int kCols = D / 32;
+    typedef typename Cols<kCols>::type V;
     griddep_wait();
+    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
     const PlanHead h = *(const PlanHead*)a.ws;
     const unsigned* cum = (const unsigned*)(a.ws + 256);
-    const long long id = (long long)blockIdx.x * kRows + threadIdx.x / L;
-    const int lane = threadIdx.x % L;
-    const int tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
     if (tok >= (int)h.tokens) return;
     const int b = request_of(a, tok);
-    const Req r = request(a, b, nullptr);
+    const Req r = request(a, b);
     const int j = tok - r.first;
     if (j < 0 || j >= r.n) return;
     const int kv = head / a.G, hg = head - kv * a.G;
 
-    float M = -INFINITY, Ls = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float m, float l, const float4& v) {  // one more piece: m = -inf, l = 0 leaves everything as it is
-        const float mn = m > M ? m : M;
-        const float f = M == mn ? 1.f : ex2(M - mn), g = m == mn ? (l == 0.f ? 0.f : 1.f) : (l == 0.f ? 0.f : ex2(m - mn));
-        M = mn;
-        Ls = Ls * f + l * g;
-        o.x = o.x * f + v.x * g;
-        o.y = o.y * f + v.y * g;
-        o.z = o.z * f + v.z * g;
-        o.w = o.w * f + v.w * g;
-    };
-    // all pieces of the item whose first step is `first`, for its block row `rr`
+    float M = -INFINITY, Ls = 0.f, o[kCols];
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) o[i] = 0.f;
+    // all pieces of the item whose first step is `first`, for its block row `rr`: two candidates a CTA (its parts), one
+    // candidate a lane
     auto item = [&](unsigned first, unsigned tiles, int rows, int index, int rr, const unsigned char* base, int R) {
         const int sh = rows > kTile ? 1 : 0;
-        const unsigned len = tiles << sh;
+        const unsigned len = (tiles << sh) + kItemSteps;
         const int c0 = cta_of(first, h.total, a.ctas), c1 = cta_of(first + len - 1, h.total, a.ctas);
         const long long part = part_bytes(R, D);
         const int row = rr & (kTile - 1), half = rr >> 7;
-        for (int c = c0; c <= c1; ++c) {
-            const unsigned lo = max(range_lo(h.total, c, a.ctas), first), hi = min(range_lo(h.total, c + 1, a.ctas), first + len);
-            if (hi <= lo) continue;
-            const unsigned t0 = (lo - first + sh) >> sh, t1 = (hi - first + sh) >> sh;
-            if (t1 <= t0) continue;
-            const unsigned char* slot = base + (long long)(index + c) * 2 * part;
-            const int n = sh ? 1 : min(t1 - t0, 2u);
-            for (int s = 0; s < n; ++s) {
-                const float* src = (const float*)(slot + (sh ? half : s) * part);
-                const float4 v = ((const float4*)src)[lane * R + row];
-                add(src[(long long)R * D + row], src[(long long)R * D + R + row], v);
+        const int lanes = sh ? 32 : 16;  // CTAs looked up at once
+        for (int cb = c0; cb <= c1; cb += lanes) {
+            const int c = cb + (sh ? lane : lane >> 1), s = sh ? half : lane & 1;
+            float m = -INFINITY, l = 0.f;
+            const float* src = nullptr;
+            if (c <= c1) {
+                const unsigned lo = max(range_lo(h.total, c, a.ctas), first), hi = min(range_lo(h.total, c + 1, a.ctas), first + len);
+                unsigned t0 = 0, t1 = 0;
+                if (hi > lo) tiles_of(lo - first, hi - first, sh, t0, t1);
+                if (t1 > t0 + (sh ? 0 : s)) {
+                    src = (const float*)(base + ((long long)(index + c) * 2 + s) * part);
+                    m = src[(long long)R * D + row];
+                    l = src[(long long)R * D + R + row];
+                }
+            }
+            const float mn = fmaxf(M, warp_max(m));
+            const float f = M == mn ? 1.f : ex2(M - mn);                      // of what is there
+            const float g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
+            M = mn;
+            Ls = Ls * f + warp_sum(l * g);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) o[i] *= f;
+            unsigned there = __ballot_sync(0xffffffffu, l != 0.f);
+            while (there != 0u) {
+                V v[4];
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int from = there != 0u ? __ffs(there) - 1 : 0;
+                    const bool on = there != 0u;
+                    there &= there - 1;
+                    const float* at = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, from);
+                    w[i] = __shfl_sync(0xffffffffu, g, from);
+                    if (on) v[i] = *(const V*)(at + ((long long)(lane * kCols >> 2) * R + row) * 4 + (lane * kCols & 3));
+                    else w[i] = 0.f, v[i] = V();
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float* e = (const float*)&v[i];
+#pragma unroll
+                    for (int k = 0; k < kCols; ++k) o[k] += e[k] * w[i];
+                }
             }
         }
     };
     if (h.tiles > 0) {
         const int total = (int)h.tokens * a.G, gr = tok * a.G + hg, rb = gr / (2 * kTile), blocks = row_blocks(total);
-        item(kv * h.per_head + rb * 2 * h.tiles, h.tiles, min(2 * kTile, total - rb * 2 * kTile), kv * blocks + rb, gr - rb * 2 * kTile,
+        item(kv * h.per_head + rb * (2 * h.tiles + kItemSteps), h.tiles, min(2 * kTile, total - rb * 2 * kTile), kv * blocks + rb, gr - rb * 2 * kTile,
              a.ws + a.ws_prefix, kTile);
     }
     const unsigned tiles = own_tiles(a, r, (int)h.prefix);
     if (tiles > 0) {
         const int total = r.n * a.G, gr = j * a.G + hg, rb = gr / (2 * kTile), blocks = row_blocks(total);
-        const unsigned per_head = tiles * steps_of_rows(total);
-        item(cum[b] + kv * per_head + rb * 2 * tiles, tiles, min(2 * kTile, total - rb * 2 * kTile), (int)cum[a.batch + b] + kv * blocks + rb,
-             gr - rb * 2 * kTile, a.ws + a.ws_suffix, a.suffix_rows);
+        item(cum[b] + kv * head_steps(tiles, total) + rb * (2 * tiles + kItemSteps), tiles, min(2 * kTile, total - rb * 2 * kTile),
+             (int)cum[a.batch + b] + kv * blocks + rb, gr - rb * 2 * kTile, a.ws + a.ws_suffix, a.suffix_rows);
     }
     const float inv = Ls == 0.f ? 0.f : 1.f / Ls;  // a row that saw no key is zero
-    uint2 w;
-    w.x = pack2<kHalf>(o.x * inv, o.y * inv);
-    w.y = pack2<kHalf>(o.z * inv, o.w * inv);
-    *(uint2*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * 4) * 2) = w;
+    uint32_t w[kCols / 2];
+#pragma unroll
+    for (int i = 0; i < kCols / 2; ++i) w[i] = pack2<kHalf>(o[2 * i] * inv, o[2 * i + 1] * inv);
+    uint32_t* out = (uint32_t*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * kCols) * 2);
+    if (kCols == 4) *(uint2*)out = make_uint2(w[0], w[kCols / 2 - 1]);
+    else *out = w[0];
     if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + log2f(Ls)) * kLn2;
 }
 
 template <int D, bool kHalf>
-static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t s, bool pdl) {
+static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const PrefixAttnMaps& maps, cudaStream_t s, bool pdl) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -813,19 +952,18 @@ static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const CUtensorMap& k
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_attn_kernel<D, kHalf>, a, k, v);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_attn_kernel<D, kHalf>, a, maps);
     if (e != cudaSuccess) return e;
-    constexpr int rows = 256 / (D / 4);
-    cfg.gridDim = dim3((unsigned)(((long long)a.rows * a.qh + rows - 1) / rows));
+    cfg.gridDim = dim3((unsigned)(((long long)a.rows * a.qh + 7) / 8));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;  // its wait is its first statement, so it may always start under the first kernel's tail
     return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf>, a);
 }
 
-cudaError_t prefix_attn_launch(const PrefixAttnArgs& a, const CUtensorMap& k, const CUtensorMap& v, int dim, bool fp16, cudaStream_t s, bool pdl) {
-    if (dim == 64) return fp16 ? prefix_attn_run<64, true>(a, k, v, s, pdl) : prefix_attn_run<64, false>(a, k, v, s, pdl);
-    return fp16 ? prefix_attn_run<128, true>(a, k, v, s, pdl) : prefix_attn_run<128, false>(a, k, v, s, pdl);
+cudaError_t prefix_attn_launch(const PrefixAttnArgs& a, const PrefixAttnMaps& maps, int dim, bool fp16, cudaStream_t s, bool pdl) {
+    if (dim == 64) return fp16 ? prefix_attn_run<64, true>(a, maps, s, pdl) : prefix_attn_run<64, false>(a, maps, s, pdl);
+    return fp16 ? prefix_attn_run<128, true>(a, maps, s, pdl) : prefix_attn_run<128, false>(a, maps, s, pdl);
 }
 
 cudaError_t prefix_attn_prepare() {

@@ -98,7 +98,7 @@ struct MkLaunch {
     mk::RopeTableArgs rope_table;
     mk::RotaryArgs rotary;
     mk::PrefixAttnArgs pattn;
-    CUtensorMap k_map, v_map;
+    mk::PrefixAttnMaps maps;
     int head_dim;
     bool fp16, interleaved;
     // the DFlash2 draft's launch lists: n_dops > 0 replaces both of the above
@@ -974,7 +974,7 @@ static int run_ops(const MkLaunch* L, cudaStream_t s, bool pdl) {
             case OP_BLOCK_TABLES: e = block_tables_launch(L->tables, L->sms, s, pdl); break;
             case OP_ROPE_TABLE: e = rope_table_launch(L->rope_table, L->sms, s, pdl); break;
             case OP_ROTARY: e = rotary_launch(L->rotary, L->fp16, L->interleaved, s, pdl); break;
-            case OP_PREFIX_ATTN: e = prefix_attn_launch(L->pattn, L->k_map, L->v_map, L->head_dim, L->fp16, s, pdl); break;
+            case OP_PREFIX_ATTN: e = prefix_attn_launch(L->pattn, L->maps, L->head_dim, L->fp16, s, pdl); break;
             default: return fail("op %d does not exist", L->op_kind[i]);
         }
         if (e != cudaSuccess) return fail("op %d launch: %s", L->op_kind[i], cudaGetErrorString(e));
