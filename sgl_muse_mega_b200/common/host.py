@@ -224,10 +224,13 @@ class Module:
 class Launch:
     def __init__(self, lib: Library, handle, module):
         self.lib, self.handle, self.module = lib, handle, module
+        self.enqueue = lib.dll.mk_launch  # looked up once: a step makes hundreds of these calls
         _free_with(self, lib.dll.mk_launch_free, handle)
 
     def __call__(self, stream: int, pdl: bool = False) -> None:
-        self.lib.check(self.lib.dll.mk_launch(self.handle, stream, int(pdl)), "mk_launch")
+        rc = self.enqueue(self.handle, stream, pdl)
+        if rc != 0:
+            self.lib.check(rc, "mk_launch")
 
     def step(self, stream: int, first: int, count: int) -> None:
         self.lib.check(self.lib.dll.mk_launch_step(self.handle, stream, first, count), "mk_launch_step")

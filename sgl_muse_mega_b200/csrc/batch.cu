@@ -197,45 +197,36 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Bloc
 // ---- rope table -----------------------------------------------------------------------------------------------------
 // out[r] = {cos(pos f_i) | sin(pos f_i)} mult, pos = first + r. Angles are held in turns in 64 bits (pos f_i / 2 pi less its
 // whole part, exact to 2^-52 of the angle), because a far position times a frequency keeps too few bits of its fraction
-// in 32. A 64-bit sine pair costs about a hundred double operations, so a CTA evaluates it only for kHi block starts and
-// kLo offsets of each frequency and forms its kHi x kLo positions by the addition theorem: four double operations a pair,
-// error about 2^-52 against the 2^-24 of the result's own rounding.
-template <int kHi, int kLo>
-__global__ void __launch_bounds__(256) rope_table_kernel(const RopeTableArgs a) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    const int F = a.rot / 2;
-    double2* hi = (double2*)smem;   // [kHi][F]
-    double2* lo = hi + kHi * F;     // [kLo][F]
-    const long long r0 = (long long)blockIdx.x * (kHi * kLo);
-    for (int i = threadIdx.x; i < (kHi + kLo) * F; i += 256) {
-        const int e = i / F, f = i - e * F;
-        const long long pos = e < kHi ? a.first + r0 + (long long)e * kLo : (long long)(e - kHi);
-        const double t = (double)pos * a.turns[f];
-        double sn, cs;
-        sincospi(2.0 * (t - rint(t)), &sn, &cs);
-        hi[i] = e < kHi ? make_double2(cs * a.mult, sn * a.mult) : make_double2(cs, sn);
+// in 32. A 64-bit sine pair costs about a hundred double operations, so a thread evaluates it once for kRows positions of a
+// frequency and turns on from one position to the next by the addition theorem with the pair of a single step (from the
+// host): four double operations a pair, error at most kRows 2^-52 against the 2^-24 of the result's own rounding.
+template <int kRows>
+__global__ void __launch_bounds__(128) rope_table_kernel(const RopeTableArgs a) {
+    const int F = a.rot / 2, groups = F / 4;  // a thread: four neighbouring frequencies of kRows positions
+    const long long id = (long long)blockIdx.x * 128 + threadIdx.x;
+    const int f = (int)(id % groups) * 4;
+    const long long r0 = id / groups * kRows;
+    double c[4], s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const double t = (double)(a.first + r0) * a.turns[f + j];
+        sincospi(2.0 * (t - rint(t)), &s[j], &c[j]);
+        c[j] *= a.mult;
+        s[j] *= a.mult;
     }
-    __syncthreads();
     griddep_wait();
-    const int groups = F / 4;  // a thread: four frequencies of kLo positions
-    for (int i = threadIdx.x; i < kHi * groups; i += 256) {
-        const int h = i / groups, f = (i - h * groups) * 4;
-        double2 H[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) H[j] = hi[h * F + f + j];
-        float* out = a.out + (r0 + (long long)h * kLo) * a.rot + f;
+    float* out = a.out + r0 * a.rot + f;
 #pragma unroll 4
-        for (int l = 0; l < kLo; ++l) {
-            if (r0 + h * kLo + l >= a.rows) break;
-            float c[4], s[4];
+    for (int l = 0; l < kRows; ++l) {
+        if (r0 + l >= a.rows) return;
+        *(float4*)out = make_float4((float)c[0], (float)c[1], (float)c[2], (float)c[3]);
+        *(float4*)(out + F) = make_float4((float)s[0], (float)s[1], (float)s[2], (float)s[3]);
+        out += a.rot;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double2 L = lo[l * F + f + j];
-                c[j] = (float)(H[j].x * L.x - H[j].y * L.y);
-                s[j] = (float)(H[j].y * L.x + H[j].x * L.y);
-            }
-            *(float4*)(out + (long long)l * a.rot) = make_float4(c[0], c[1], c[2], c[3]);
-            *(float4*)(out + (long long)l * a.rot + F) = make_float4(s[0], s[1], s[2], s[3]);
+        for (int j = 0; j < 4; ++j) {
+            const double cs = a.step[f + j].x, sn = a.step[f + j].y, x = c[j];
+            c[j] = x * cs - s[j] * sn;
+            s[j] = s[j] * cs + x * sn;
         }
     }
 }
@@ -302,50 +293,66 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     const int turn = kInter ? a.rot / N : half / N, pieces = turn + (a.dim - a.rot) / N;
     const int step = blockDim.x / pieces, c = threadIdx.x % pieces;
     if ((int)threadIdx.x < step * pieces) {
+        constexpr int kHeads = 3;  // heads in flight a thread: their loads go out before the table row is needed
+        const bool turned = c < turn;
+        const int at = turned ? c * N : a.rot + (c - turn) * N;
         float cs[N], sn[N];
-        if (c < turn) {
-            constexpr int n = kInter ? N / 2 : N;
+        bool have = false;
+        for (int h0 = threadIdx.x / pieces; h0 < a.qh + a.kvh; h0 += kHeads * step) {
+            W w0[kHeads], w1[kHeads];
 #pragma unroll
-            for (int j = 0; j < n; j += 2) {
-                const float2 x = *(const float2*)(tab + c * n + j), y = *(const float2*)(tab + half + c * n + j);
-                cs[j] = x.x, cs[j + 1] = x.y;
-                sn[j] = a.inverse ? -y.x : y.x, sn[j + 1] = a.inverse ? -y.y : y.y;
-            }
-        }
-        const int at = c < turn ? c * N : a.rot + (c - turn) * N;
-        auto put = [&](bool isq, int h, int d, const W& w) {
-            if (isq) *(W*)(qo + h * a.qo_head + d) = w;
-            else {
-                if (ko != nullptr) *(W*)(ko + h * a.ko_head + d) = w;
-                if (kc != nullptr) *(W*)(kc + h * a.kc_head + d) = w;
-            }
-        };
-        for (int hh = threadIdx.x / pieces; hh < a.qh + a.kvh; hh += step) {
-            const bool isq = hh < a.qh;
-            const int h = isq ? hh : hh - a.qh;
-            const T* src = isq ? qr + h * a.q_head : kr + h * a.k_head;
-            W w0 = *(const W*)(src + at), w1;
-            T2* x0 = (T2*)&w0;
-            T2* x1 = (T2*)&w1;
-            if (c < turn) {
-                if (kInter) {
-#pragma unroll
-                    for (int j = 0; j < N / 2; ++j) {
-                        const float2 v = P2::up(x0[j]);
-                        x0[j] = P2::down(v.x * cs[j] - v.y * sn[j], v.y * cs[j] + v.x * sn[j]);
-                    }
-                } else {
-                    w1 = *(const W*)(src + half + at);
-#pragma unroll
-                    for (int j = 0; j < N / 2; ++j) {
-                        const float2 x = P2::up(x0[j]), y = P2::up(x1[j]);
-                        x0[j] = P2::down(x.x * cs[2 * j] - y.x * sn[2 * j], x.y * cs[2 * j + 1] - y.y * sn[2 * j + 1]);
-                        x1[j] = P2::down(y.x * cs[2 * j] + x.x * sn[2 * j], y.y * cs[2 * j + 1] + x.y * sn[2 * j + 1]);
-                    }
-                    put(isq, h, half + at, w1);
+            for (int i = 0; i < kHeads; ++i) {
+                const int hh = h0 + i * step;
+                if (hh < a.qh + a.kvh) {
+                    const T* src = hh < a.qh ? qr + hh * a.q_head : kr + (hh - a.qh) * a.k_head;
+                    w0[i] = *(const W*)(src + at);
+                    if (!kInter && turned) w1[i] = *(const W*)(src + half + at);
                 }
             }
-            put(isq, h, at, w0);
+            if (!have && turned) {
+                constexpr int n = kInter ? N / 2 : N;
+#pragma unroll
+                for (int j = 0; j < n; j += 2) {
+                    const float2 x = *(const float2*)(tab + c * n + j), y = *(const float2*)(tab + half + c * n + j);
+                    cs[j] = x.x, cs[j + 1] = x.y;
+                    sn[j] = a.inverse ? -y.x : y.x, sn[j + 1] = a.inverse ? -y.y : y.y;
+                }
+            }
+            have = true;
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i) {
+                const int hh = h0 + i * step;
+                if (hh >= a.qh + a.kvh) break;
+                const bool isq = hh < a.qh;
+                const int h = isq ? hh : hh - a.qh;
+                auto put = [&](int d, const W& w) {
+                    if (isq) *(W*)(qo + h * a.qo_head + d) = w;
+                    else {
+                        if (ko != nullptr) *(W*)(ko + h * a.ko_head + d) = w;
+                        if (kc != nullptr) *(W*)(kc + h * a.kc_head + d) = w;
+                    }
+                };
+                T2* x0 = (T2*)&w0[i];
+                T2* x1 = (T2*)&w1[i];
+                if (turned) {
+                    if (kInter) {
+#pragma unroll
+                        for (int j = 0; j < N / 2; ++j) {
+                            const float2 v = P2::up(x0[j]);
+                            x0[j] = P2::down(v.x * cs[j] - v.y * sn[j], v.y * cs[j] + v.x * sn[j]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < N / 2; ++j) {
+                            const float2 x = P2::up(x0[j]), y = P2::up(x1[j]);
+                            x0[j] = P2::down(x.x * cs[2 * j] - y.x * sn[2 * j], x.y * cs[2 * j + 1] - y.y * sn[2 * j + 1]);
+                            x1[j] = P2::down(y.x * cs[2 * j] + x.x * sn[2 * j], y.y * cs[2 * j + 1] + x.y * sn[2 * j + 1]);
+                        }
+                        put(half + at, w1[i]);
+                    }
+                }
+                put(at, w0[i]);
+            }
         }
     }
     if (a.v != nullptr && slot >= 0) {
@@ -384,11 +391,11 @@ cudaError_t block_tables_launch(const BlockTablesArgs& a, int sms, cudaStream_t 
 }
 
 cudaError_t rope_table_launch(const RopeTableArgs& a, int sms, cudaStream_t s, bool pdl) {
-    const size_t F = a.rot / 2;
-    // 64 positions a CTA while 256 would leave SMs without one
-    if (a.rows < 256ll * sms)
-        return launch_batch(rope_table_kernel<8, 8>, dim3((unsigned)((a.rows + 63) / 64)), dim3(256), 16 * F * 16, s, pdl, a);
-    return launch_batch(rope_table_kernel<16, 16>, dim3((unsigned)((a.rows + 255) / 256)), dim3(256), 32 * F * 16, s, pdl, a);
+    const long long groups = a.rot / 8;
+    auto grid = [&](int rows) { return dim3((unsigned)(((a.rows + rows - 1) / rows * groups + 127) / 128)); };
+    // 16 positions a thread once that fills the SMs; 4 for short tables, whose time is one thread's chain
+    if ((a.rows + 15) / 16 * groups >= 256ll * sms) return launch_batch(rope_table_kernel<16>, grid(16), dim3(128), 0, s, pdl, a);
+    return launch_batch(rope_table_kernel<4>, grid(4), dim3(128), 0, s, pdl, a);
 }
 
 template <typename T>
@@ -409,7 +416,6 @@ cudaError_t rotary_launch(const RotaryArgs& a, bool fp16, bool interleaved, cuda
 cudaError_t batch_prepare() {
     cudaError_t e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)block_tables_smem(kMaxBatch, kMaxPoolRows));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(rope_table_kernel<16, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * (kMaxRot / 2) * 16);
     return e;
 }
 

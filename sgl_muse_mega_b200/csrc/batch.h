@@ -19,6 +19,7 @@ __device__ __forceinline__ void batch_status(int* status, int code, int where, i
 }
 
 constexpr int kMaxBatch = 4096;        // requests of a block-table or attention launch
+constexpr int kAttnCtas = 148;         // CTAs of an attention launch: one an SM
 constexpr int kMaxPoolRows = 1 << 18;  // rows of the request table (two bits each in shared memory)
 
 struct BlockTablesArgs {
@@ -49,6 +50,7 @@ struct RopeTableArgs {
     int rot;
     double mult;
     double turns[kMaxRot / 2];  // turns per position of each frequency: inv_freq / 2 pi
+    double2 step[kMaxRot / 2];  // cos and sin of one position's angle
 };
 
 struct RotaryArgs {
@@ -89,7 +91,6 @@ struct PrefixAttnArgs {
     float scale_log2;
     unsigned char* ws;
     long long ws_prefix, ws_suffix;  // byte offsets of the partials in ws
-    int ctas;
     int* status;
 };
 

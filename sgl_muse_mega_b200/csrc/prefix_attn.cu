@@ -31,11 +31,11 @@ constexpr int kTile = 128;  // rows of a step and keys of a tile
 constexpr int kAttnThreads = 384;
 constexpr float kLn2 = 0.69314718055994530942f;
 // What an item costs besides its steps (its queries in, its O out, the tensor core's start), counted in steps
-constexpr unsigned kItemSteps = 1;
+constexpr unsigned kItemSteps = 3;
 
 // ---- the plan: the same numbers in every warp of both kernels ---------------------------------------------------------
 struct PlanHead {  // in front of the scratch, for the merge kernel
-    unsigned total, prefix_steps, tiles, pad, per_head, p_lo, prefix, tokens;
+    unsigned total, tiles, per_head, prefix, tokens, pad[3];
 };
 
 struct Req {
@@ -95,33 +95,85 @@ struct Plan {
     unsigned prefix_steps, total;
 };
 
-// One warp; every lane gets the result. Two passes over the batch's lengths; all loads that open the first are issued at
-// once, the second finds them in L1 (a lane's first request stays in registers).
-__device__ Plan make_plan(const PrefixAttnArgs& a, int lane, int* status, unsigned* cum) {
+// inclusive sums over the lanes
+__device__ __forceinline__ void scan(unsigned& x, int& y, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned u = __shfl_up_sync(0xffffffffu, x, o);
+        const int v = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) x += u, y += v;
+    }
+}
+
+// The batch's lengths as a warp holds them: request b in lane b % 32. The first 128 stay in registers, requested all at once
+// when the kernel starts; later ones are read again from L1.
+struct Lens {
+    static constexpr int kHeld = 4;
+    Req r[kHeld];
+    int want, tokens;
+    __device__ __forceinline__ void load(const PrefixAttnArgs& a, int lane) {
+        want = __ldg(a.prefix_len);
+        tokens = __ldg(a.cu_rows + a.batch);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int b = min(32 * i + lane, a.batch - 1);
+            r[i].first = __ldg(a.cu_rows + b);
+            r[i].n = __ldg(a.cu_rows + b + 1);
+            r[i].len = __ldg(a.kv_lens + b);
+        }
+    }
+    // what the loads brought, as far as it is usable
+    __device__ __forceinline__ void check(const PrefixAttnArgs& a, int lane, int* status) {
+        const int cap = a.width * a.page;  // up to 2^30
+        if (want < 0 || want > cap) {
+            if (status != nullptr) batch_status(status, 4, 522, want, cap);
+            want = 0;
+        }
+        if (tokens < 0 || tokens > a.rows) {
+            if (status != nullptr) batch_status(status, 4, 523, tokens, a.rows);
+            tokens = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int b = 32 * i + lane;
+            r[i] = b < a.batch ? usable(a, b, r[i].first, r[i].n, r[i].len, status) : Req{0, 0, 0};
+        }
+    }
+    // fn(request, b) for blocks of 32 requests in order, b = the lane's request (an empty one past the batch); fn returns false
+    // to stop. Whole warps.
+    template <typename Fn>
+    __device__ __forceinline__ void each(const PrefixAttnArgs& a, int lane, Fn&& fn) const {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            if (32 * i >= a.batch) return;
+            if (!fn(r[i], 32 * i + lane)) return;
+        }
+        for (int b0 = 32 * kHeld; b0 < a.batch; b0 += 32) {
+            const int b = b0 + lane;
+            Req x{0, 0, 0};
+            if (b < a.batch) x = request(a, b);
+            if (!fn(x, b)) return;
+        }
+    }
+};
+
+// One warp; every lane gets the result. `cum`: first step and first item of each request, for the merge.
+__device__ __forceinline__ Plan make_plan(const PrefixAttnArgs& a, const Lens& lens, int lane, int* status, unsigned* cum) {
     Plan p;
-    const int cap = a.width * a.page;  // below 2^30 + page
-    const int at = min(lane, a.batch - 1);
-    int want = __ldg(a.prefix_len);
-    p.tokens = __ldg(a.cu_rows + a.batch);
-    const int c0 = __ldg(a.cu_rows + at), c1 = __ldg(a.cu_rows + at + 1), len = __ldg(a.kv_lens + at);
-    if (want < 0 || want > cap) {
-        if (status != nullptr) batch_status(status, 4, 522, want, cap);
-        want = 0;
-    }
-    if (p.tokens < 0 || p.tokens > a.rows) {
-        if (status != nullptr) batch_status(status, 4, 523, p.tokens, a.rows);
-        p.tokens = 0;
-    }
-    const Req mine = lane < a.batch ? usable(a, lane, c0, c1, len, status) : Req{0, 0, 0};
+    const int want = lens.want;
+    p.tokens = lens.tokens;
     int live = 0, ref = 0x7fffffff, lo = 0x7fffffff, hi = 0;
-    for (int b = lane; b < a.batch; b += 32) {
-        const Req r = b == lane ? mine : usable(a, b, __ldg(a.cu_rows + b), __ldg(a.cu_rows + b + 1), __ldg(a.kv_lens + b), status);
-        if (r.n <= 0 || r.len <= 0) continue;
-        ++live;
-        if (r.len >= want) ref = min(ref, b);
-        lo = min(lo, a.window > 0 ? max(0, r.len - r.n - a.window) : 0);
-        hi = max(hi, min(want, r.len));
-    }
+    lens.each(a, lane, [&](const Req& r, int b) {
+        if (status != nullptr && b >= 32 * Lens::kHeld && b < a.batch)
+            usable(a, b, __ldg(a.cu_rows + b), __ldg(a.cu_rows + b + 1), __ldg(a.kv_lens + b), status);  // to be recorded
+        if (r.n > 0 && r.len > 0) {
+            ++live;
+            if (r.len >= want) ref = min(ref, b);
+            lo = min(lo, a.window > 0 ? max(0, r.len - r.n - a.window) : 0);
+            hi = max(hi, min(want, r.len));
+        }
+        return true;
+    });
     live = __reduce_add_sync(0xffffffffu, live);
     ref = __reduce_min_sync(0xffffffffu, ref);
     lo = __reduce_min_sync(0xffffffffu, lo);
@@ -133,46 +185,45 @@ __device__ Plan make_plan(const PrefixAttnArgs& a, int lane, int* status, unsign
     p.tiles = p.prefix > 0 && hi > p.p_lo ? (unsigned)(hi - p.p_lo + kTile - 1) / kTile : 0u;
     p.per_head = head_steps(p.tiles, p.tokens * a.G);
     p.prefix_steps = p.per_head * a.kvh;
-    unsigned sum = p.prefix_steps;
+    unsigned sum = 0;
+    if (cum == nullptr) {
+        lens.each(a, lane, [&](const Req& r, int) {
+            sum += own_steps(a, r, p.prefix);
+            return true;
+        });
+        p.total = p.prefix_steps + __reduce_add_sync(0xffffffffu, sum);
+        return p;
+    }
+    sum = p.prefix_steps;
     int items = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const int b = b0 + lane;
-        Req r{0, 0, 0};
-        if (b0 == 0) r = mine;
-        else if (b < a.batch) r = request(a, b);
+    lens.each(a, lane, [&](const Req& r, int b) {
         const unsigned x = own_steps(a, r, p.prefix);
-        if (cum == nullptr) {
-            sum += __reduce_add_sync(0xffffffffu, x);
-            continue;
-        }
         const int it = own_items(a, r);
         unsigned inc = x;
         int ci = it;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
-            const int z = __shfl_up_sync(0xffffffffu, ci, o);
-            if (lane >= o) inc += y, ci += z;
-        }
-        if (b < a.batch) {  // first step and first item of each request, for the merge
+        scan(inc, ci, lane);
+        if (b < a.batch) {
             cum[b] = sum + inc - x;
             cum[a.batch + b] = (unsigned)(items + ci - it);
         }
         sum += __shfl_sync(0xffffffffu, inc, 31);
         items += __shfl_sync(0xffffffffu, ci, 31);
-    }
+        return true;
+    });
     p.total = sum;
     return p;
 }
 
-// first step of CTA c's range: floor(total c / ctas), without a 64-bit division
-__device__ __forceinline__ unsigned range_lo(unsigned total, int c, int ctas) {
-    const unsigned n = (unsigned)ctas, q = total / n;
-    return q * c + (total - q * n) * c / n;
+// The work is cut for this many CTAs (one an SM), a constant so that no division by a variable stands in front of the work.
+// No CTA waits for another, so a part with fewer SMs would only run them in turn.
+constexpr unsigned kCtas = kAttnCtas;
+__device__ __forceinline__ unsigned range_lo(unsigned total, unsigned c) {  // first step of CTA c's range: floor(total c / kCtas)
+    const unsigned q = total / kCtas;
+    return q * c + (total - q * kCtas) * c / kCtas;
 }
-__device__ __forceinline__ int cta_of(unsigned step, unsigned total, int ctas) {  // whose range holds the step
-    if (total < (1u << 24)) return (int)(((step + 1) * (unsigned)ctas - 1) / total);  // ctas <= 148 < 2^8
-    return (int)((((unsigned long long)step + 1) * ctas - 1) / total);
+__device__ __forceinline__ int cta_of(unsigned step, unsigned total) {  // whose range holds the step
+    if (total < (1u << 24)) return (int)(((step + 1) * kCtas - 1) / total);  // kCtas < 2^8
+    return (int)((((unsigned long long)step + 1) * kCtas - 1) / total);
 }
 
 // An item's piece in one CTA's range
@@ -202,9 +253,9 @@ struct Walker {
     unsigned tiles;
     int row_total, blocks, key0;
 
-    __device__ Walker(const PrefixAttnArgs& a_, const Plan& p_, int cta, int lane) : a(a_), p(p_) {
-        unsigned pos = range_lo(p.total, cta, a.ctas);
-        left = range_lo(p.total, cta + 1, a.ctas) - pos;
+    __device__ __forceinline__ Walker(const PrefixAttnArgs& a_, const Plan& p_, const Lens& lens, int cta, int lane) : a(a_), p(p_) {
+        unsigned pos = range_lo(p.total, cta);
+        left = range_lo(p.total, cta + 1) - pos;
         b = -1;
         items = 0;
         h = rb = 0;
@@ -213,31 +264,24 @@ struct Walker {
         if (left == 0) return;
         if (pos >= p.prefix_steps) {  // starts in a request's items: find it, the whole warp together
             unsigned sum = p.prefix_steps;
-            for (int b0 = 0; b0 < a.batch; b0 += 32) {
-                const int bb = b0 + lane;
-                Req q{0, 0, 0};
-                if (bb < a.batch) q = request(a, bb);
+            lens.each(a, lane, [&](const Req& q, int bb) {
                 const unsigned x = own_steps(a, q, p.prefix);
                 const int it = own_items(a, q);
                 unsigned inc = x;
                 int ci = it;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned y = __shfl_up_sync(0xffffffffu, inc, o);
-                    const int z = __shfl_up_sync(0xffffffffu, ci, o);
-                    if (lane >= o) inc += y, ci += z;
-                }
+                scan(inc, ci, lane);
                 const unsigned hit = __ballot_sync(0xffffffffu, pos < sum + inc);
+                const int l = hit != 0u ? __ffs(hit) - 1 : 31;
                 if (hit != 0u) {
-                    const int l = __ffs(hit) - 1;
-                    b = b0 + l;
+                    b = bb - lane + l;
                     pos -= sum + __shfl_sync(0xffffffffu, inc - x, l);
                     items += __shfl_sync(0xffffffffu, ci - it, l);
-                    break;
+                    return false;
                 }
                 sum += __shfl_sync(0xffffffffu, inc, 31);
                 items += __shfl_sync(0xffffffffu, ci, 31);
-            }
+                return true;
+            });
         }
         load();
         const unsigned per_head = head_steps(tiles, row_total), block = 2 * tiles + kItemSteps;
@@ -310,7 +354,7 @@ struct Cfg {
 struct Bars {
     uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[4], q_empty[4];
     uint64_t s_full[2], s_free[2], p_ready[2], o_full[2], pv_done[2];
-    uint64_t drain;
+    uint64_t drain[2];
     uint32_t tmem;
     int abort;
 };
@@ -401,6 +445,32 @@ __device__ __forceinline__ float2 add2(float2 x, float2 y) {
         : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
     return r;
 }
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+// 2^x for two x >= -126 on the FMA pipe: x = k + f with k the nearest whole number, 2^f on [-1/2, 1/2] by the polynomial of
+// degree 4 with the least relative error (2.7e-6; exchange algorithm), k added to the exponent. The special-function unit
+// gives 16 results a clock and SM, which bounds the softmax of 64-wide heads; kPolyOf8 of 8 results come from here.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 r = add2(x, magic);  // k in the low bits
+    const float2 f = fma2(add2(r, back), make_float2(-1.f, -1.f), x);
+    float2 p = fma2(f, make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f), make_float2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    p = fma2(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    p = fma2(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    p = fma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+}
+constexpr int kPolyOf8 = 3;
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
@@ -411,6 +481,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // Called by whole warps; one expired wait ends every role of the CTA.
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, Bars* s, int* status, int where) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     const bool ok = mbar_wait(bar, parity, &s->abort);
     if (__all_sync(0xffffffffu, ok)) return true;  // the whole warp goes the same way
     if (!ok && atomicExch(&s->abort, 1) == 0) batch_status(status, 3, where, 0, 0);
@@ -424,6 +495,18 @@ __device__ __forceinline__ int request_of(const PrefixAttnArgs& a, int t) {
         const int mid = (lo + hi) >> 1;
         if (__ldg(a.cu_rows + mid) <= t) lo = mid;
         else hi = mid;
+    }
+    return lo;
+}
+// the same by a whole warp for one token: 32 probes a round
+__device__ __forceinline__ int request_of_warp(const PrefixAttnArgs& a, int t, int lane) {
+    int lo = 0, n = a.batch;  // the last b in [lo, lo + n) with cu[b] <= t
+    while (n > 1) {
+        const int step = (n + 31) / 32, b = lo + lane * step;
+        const bool le = lane * step < n && (lane == 0 || __ldg(a.cu_rows + b) <= t);
+        const int last = 31 - __clz(__ballot_sync(0xffffffffu, le));
+        lo += last * step;
+        n = min(step, n - last * step);
     }
     return lo;
 }
@@ -458,6 +541,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     unsigned char* Vs = Ks + C::kRing * C::kTileBytes;
     unsigned char* Qs = Vs + C::kRing * C::kTileBytes;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    griddep_wait();
+    Lens lens;
+    lens.load(a, lane);  // under the set-up below
+    if (warp == 9 && lane < 5) {
+        const CUtensorMap* m = lane == 0 ? &maps.k_run : lane == 1 ? &maps.v_run : lane == 2 ? &maps.k_row : lane == 3 ? &maps.v_row : &maps.q;
+        if (lane < 4 || a.q_box) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(&S.k_full[i], 1);
@@ -474,7 +564,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             mbar_init(&S.o_full[i], 1);
             mbar_init(&S.pv_done[i], 1);
         }
-        mbar_init(&S.drain, 1);
+        mbar_init(&S.drain[0], 1);
+        mbar_init(&S.drain[1], 1);
         S.abort = 0;
         mbar_fence_init();
     }
@@ -483,18 +574,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t*)&S.tmem;
-    griddep_wait();
 
     unsigned* cum = (unsigned*)(a.ws + 256);
     const bool writer = blockIdx.x == 0 && warp == 0;
-    const Plan p = make_plan(a, lane, writer ? a.status : nullptr, writer ? cum : nullptr);
-    if (writer && lane == 0)
-        *(PlanHead*)a.ws = PlanHead{p.total, p.prefix_steps, p.tiles, 0u, p.per_head, (unsigned)p.p_lo, (unsigned)p.prefix,
-                                    (unsigned)p.tokens};
-    Walker walk(a, p, blockIdx.x, lane);
+    lens.check(a, lane, writer ? a.status : nullptr);
+    const Plan p = make_plan(a, lens, lane, writer ? a.status : nullptr, writer ? cum : nullptr);
+    if (writer && lane == 0) *(PlanHead*)a.ws = PlanHead{p.total, p.tiles, p.per_head, (unsigned)p.prefix, (unsigned)p.tokens, 0u, 0u, 0u};
+    Walker walk(a, p, lens, blockIdx.x, lane);
     Piece x;
     const int cap = a.width * a.page;
-    unsigned issued = 0, q_boxes = 0;  // tiles that this warp's copies were asked for
+    unsigned issued = 0, q_count = 0;  // tiles that this warp has asked for
 
     if (warp < 8) {
         // ---- softmax ----
@@ -506,15 +595,24 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         uint32_t s_par = 0, o_par = 0, pv_par = 1;  // pv: the wait for the step before the first returns at once
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
         bool ok = true;
-        while (ok && walk.next(x)) {
-            const unsigned ns = x.steps(), sub = (wg - g) & 1;
-            g += ns;
-            if (sub >= ns) continue;
+        int lo = 0, hi = 0, rr = 0;
+        unsigned ns = 0, sub = 0;
+        auto advance = [&]() -> bool {  // the next piece in which this warpgroup has steps
+            while (walk.next(x)) {
+                ns = x.steps();
+                sub = (wg - g) & 1;
+                g += ns;
+                if (sub >= ns) continue;
+                rr = row + (x.pair() ? (int)sub * kTile : 0);
+                row_keys(a, p, x, rr, lo, hi);
+                return true;
+            }
+            return false;
+        };
+        bool more = advance();
+        while (more) {
             const bool pair = x.pair();
-            const int rr = row + (pair ? (int)sub * kTile : 0);
             const bool busy = (rr & ~31) < x.rows;  // this warp has rows
-            int lo, hi;
-            row_keys(a, p, x, rr, lo, hi);
             float m = -INFINITY, l = 0.f;
             for (unsigned st = sub; st < ns; st += 2) {
                 const int kb = x.key0 + (int)(x.t0 + (pair ? st >> 1 : st)) * kTile;
@@ -533,18 +631,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     if (lane == 0) mbar_arrive(&S.s_free[wg]);
                 }
                 if (busy) {
-                    if (!__all_sync(0xffffffffu, (lo <= kb && hi >= kb + kTile) || rr >= x.rows)) {
+                    const bool whole = __all_sync(0xffffffffu, (lo <= kb && hi >= kb + kTile) || rr >= x.rows);
+                    if (!whole) {
                         const int c0 = lo - kb, c1 = hi - kb;
 #pragma unroll
                         for (int i = 0; i < 128; ++i) s[i] = i >= c0 && i < c1 ? s[i] : -INFINITY;
                     }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int i = 0; i < 128; i += 8) {
+                    for (int i = 4; i < 124; i += 8) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], fmaxf(s[i + j], s[i + 4 + j]));
+                        for (int j = 0; j < 4; ++j) mx[j] = max_nan(mx[j], max_nan(s[i + j], s[i + 4 + j]));
                     }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mx[j] = max_nan(mx[j], s[124 + j]);
+                    const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.scale_log2;
+                    if (!(top < INFINITY)) l = NAN;  // a score that is NaN or +inf: so is the row's softmax
                     // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
                     // P's type and the f32 sums carry without loss), so O is seldom rescaled.
                     const bool grow = top > m + 8.f;
@@ -569,19 +671,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     const float ms = m == -INFINITY ? 0.f : m;
                     const float2 neg = make_float2(-ms, -ms);
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    auto probabilities = [&](auto poly) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t u[16];
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t u[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            float2 e = fma2(make_float2(s[32 * i + 2 * j], s[32 * i + 2 * j + 1]), scale2, neg);
-                            e.x = ex2(e.x);
-                            e.y = ex2(e.y);
-                            sum[j & 1] = add2(sum[j & 1], e);
-                            u[j] = pack2<kHalf>(e.x, e.y);
+                            for (int j = 0; j < 16; ++j) {
+                                float2 e = fma2(make_float2(s[32 * i + 2 * j], s[32 * i + 2 * j + 1]), scale2, neg);
+                                if (j % 8 < decltype(poly)::value) e = exp2_poly(e);
+                                else e = make_float2(ex2(e.x), ex2(e.y));
+                                sum[j & 1] = add2(sum[j & 1], e);
+                                u[j] = pack2<kHalf>(e.x, e.y);
+                            }
+                            tmem_st16(tP + 16 * i, u);
                         }
-                        tmem_st16(tP + 16 * i, u);
-                    }
+                    };
+                    if (whole) probabilities(Int<kPolyOf8>());
+                    else probabilities(Int<0>());  // masked scores are -inf and their probabilities exactly 0
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     tmem_st_wait();
                     tc_fence_before();
@@ -591,14 +697,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 if (lane == 0) mbar_arrive(&S.p_ready[wg]);
             }
             if (!ok) break;
+            // while the last product runs: where this piece goes, and the next one
+            const int R = x.b < 0 ? kTile : a.suffix_rows;
+            unsigned char* dst =
+                a.ws + (x.b < 0 ? a.ws_prefix : a.ws_suffix) + ((long long)(x.index + (int)blockIdx.x) * 2 + sub) * part_bytes(R, D);
+            const bool mine = rr < x.rows;
+            more = advance();
             if (!(ok = attn_wait(&S.o_full[wg], o_par, &S, a.status, 531))) break;
             o_par ^= 1;
             if (busy) {
                 tc_fence_after();
-                const int R = x.b < 0 ? kTile : a.suffix_rows;
-                const long long part = part_bytes(R, D);
-                unsigned char* dst = a.ws + (x.b < 0 ? a.ws_prefix : a.ws_suffix) + ((long long)(x.index + (int)blockIdx.x) * 2 + sub) * part;
-                const bool mine = rr < x.rows;
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) {
                     float o[32];
@@ -619,95 +727,87 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
         }
     } else if (warp == 8) {
-        // ---- tensor core ----
+        // ---- S = Q K^T ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        // The S product of step n + 2 comes before the P V product of step n where P has columns of its own (it waits for the
-        // scores of step n to have left S), behind it and after its end where P lies over S. One cursor over the pieces makes S
-        // steps, their flags wait in a queue of two for the P V side.
-        constexpr uint32_t id_s = idesc_f16(kHalf, false, kTile), id_o = idesc_f16(kHalf, true, D);
-        unsigned ks = 0, vs = 0, qs = 0;  // running tile counts of the rings
-        unsigned queue0 = 0, queue1 = 0;  // bit 0 accumulate, 1 last of the warpgroup, 2 releases V
-        unsigned n_s = 0, st = 0, ns = 0;
-        bool have = false, ok = true;
-        // what the issuing thread hands to the tensor core is made uniform over the warp first (shuffles from lane 0): the
-        // compiler then keeps descriptors in uniform registers
-        const uint64_t q_desc = desc_sw128(smem_u32(Qs)), k_desc = desc_sw128(smem_u32(Ks)), v_desc = desc_v(smem_u32(Vs));
-        auto issue_s = [&]() -> bool {  // the next S step if there is one
-            if (!have || st == ns) {
-                if (have) qs += x.pair() ? 2 : 1;
-                have = walk.next(x);
-                if (!have) return true;
-                st = 0;
-                ns = x.steps();
-            }
+        constexpr uint32_t id_s = idesc_f16(kHalf, false, kTile);
+        // What the issuing thread hands to the tensor core is made uniform over the warp first (shuffles from lane 0): the
+        // compiler then keeps descriptors in uniform registers.
+        const uint64_t q_desc = desc_sw128(smem_u32(Qs)), k_desc = desc_sw128(smem_u32(Ks));
+        unsigned n = 0, ki = 0, kpar = 0, qi = 0, qpar = 0;  // step; ring places and their phases
+        bool ok = true;
+        while (ok && walk.next(x)) {
             const bool pair = x.pair();
-            const unsigned q = qs + (pair ? st & 1 : 0);
-            const int qi = __shfl_sync(0xffffffffu, (int)(q % C::kQ), 0), ki = __shfl_sync(0xffffffffu, (int)(ks % C::kRing), 0);
-            const int w = __shfl_sync(0xffffffffu, (int)(n_s & 1), 0);
-            const unsigned f = __shfl_sync(0xffffffffu, (st >= 2 ? 1u : 0u) | (st + 2 >= ns ? 2u : 0u) | ((!pair || (st & 1)) ? 4u : 0u) |
-                                                            (st + (pair ? 2 : 1) >= ns ? 8u : 0u), 0);
-            if (st < (pair ? 2u : 1u)) {
-                if (!attn_wait(&S.q_full[qi], (q / C::kQ) & 1, &S, a.status, 532)) return false;
-            }
-            if (!pair || !(st & 1)) {
-                if (!attn_wait(&S.k_full[ki], (ks / C::kRing) & 1, &S, a.status, 533)) return false;
-            }
-            tc_fence_after();
-            if (elect_one()) {
-                const uint64_t qd = q_desc + (uint64_t)(qi * (C::kTileBytes >> 4)), kd = k_desc + (uint64_t)(ki * (C::kTileBytes >> 4));
+            const unsigned ns = x.steps(), tiles_q = pair ? 2 : 1;
+            for (unsigned st = 0; st < ns; ++st, ++n) {
+                const int w = __shfl_sync(0xffffffffu, (int)(n & 1), 0);
+                unsigned qq = qi + (pair ? st & 1 : 0), qp = qpar;
+                if (qq >= C::kQ) qq -= C::kQ, qp ^= 1;
+                const int qs = __shfl_sync(0xffffffffu, (int)qq, 0), ks = __shfl_sync(0xffffffffu, (int)ki, 0);
+                const bool last_k = !pair || (st & 1);
+                if (st < tiles_q && !(ok = attn_wait(&S.q_full[qs], qp, &S, a.status, 532))) break;
+                if ((!pair || !(st & 1)) && !(ok = attn_wait(&S.k_full[ks], kpar, &S, a.status, 533))) break;
+                // the scores of step n - 2 have left S (where P lies over S: its P V product has ended)
+                if (!(ok = attn_wait(C::kAlias ? &S.pv_done[w] : &S.s_free[w], ((n >> 1) & 1) ^ 1, &S, a.status, 536))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t qd = q_desc + (uint64_t)(qs * (C::kTileBytes >> 4)), kd = k_desc + (uint64_t)(ks * (C::kTileBytes >> 4));
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t o = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-                    mma_ss(tmem + C::kS + w * 128, qd + o, kd + o, id_s, k > 0);
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint64_t o = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+                        mma_ss(tmem + C::kS + w * 128, qd + o, kd + o, id_s, k > 0);
+                    }
+                    tc_commit(&S.s_full[w]);
+                    if (last_k) tc_commit(&S.k_empty[ks]);
+                    if (st + tiles_q >= ns) tc_commit(&S.q_empty[qs]);
                 }
-                tc_commit(&S.s_full[w]);
-                if (f & 4u) tc_commit(&S.k_empty[ki]);
-                if (f & 8u) tc_commit(&S.q_empty[qi]);
+                __syncwarp();
+                if (last_k && ++ki == C::kRing) ki = 0, kpar ^= 1;
             }
-            __syncwarp();
-            if (w) queue1 = f;
-            else queue0 = f;
-            if (f & 4u) ++ks;
-            ++st;
-            ++n_s;
-            return true;
-        };
-        ok = issue_s() && issue_s();
-        for (unsigned n = 0; ok && n < n_s; ++n) {
-            const int w = __shfl_sync(0xffffffffu, (int)(n & 1), 0);
-            const uint32_t par = (n >> 1) & 1;  // every warpgroup barrier completes once a step
-            const unsigned f = __shfl_sync(0xffffffffu, w ? queue1 : queue0, 0);
-            const int vi = __shfl_sync(0xffffffffu, (int)(vs % C::kRing), 0);
-            if (!C::kAlias) {
-                if (!(ok = attn_wait(&S.s_free[w], par, &S, a.status, 536))) break;
-                if (!(ok = issue_s())) break;
-            }
-            if (!(ok = attn_wait(&S.v_full[vi], (vs / C::kRing) & 1, &S, a.status, 534))) break;
-            if (!(ok = attn_wait(&S.p_ready[w], par, &S, a.status, 535))) break;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint64_t vd = v_desc + (uint64_t)(vi * (C::kTileBytes >> 4));
-#pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
-                    mma_ts(tmem + C::kO + w * C::kOStep, tmem + C::kP + w * C::kPStep + 8 * k, vd + (uint64_t)(k * 2048 >> 4), id_o, k > 0 ? 1u : f & 1u);
-                tc_commit(&S.pv_done[w]);
-                if (f & 4u) tc_commit(&S.v_empty[vi]);
-                if (f & 2u) tc_commit(&S.o_full[w]);
-            }
-            __syncwarp();
-            if (f & 4u) ++vs;
-            if (C::kAlias) {
-                if (!(ok = attn_wait(&S.pv_done[w], par, &S, a.status, 536))) break;
-                ok = issue_s();
-            }
+            qi += tiles_q;
+            if (qi >= C::kQ) qi -= C::kQ, qpar ^= 1;
         }
         // the tensor core has to be done before its memory is given back
-        if (elect_one()) tc_commit(&S.drain);
+        if (elect_one()) tc_commit(&S.drain[0]);
         __syncwarp();
-        for (uint32_t i = 0; i < kWaitPolls && !mbar_try_wait(&S.drain, 0); ++i) {
+        for (uint32_t i = 0; i < kWaitPolls && !mbar_try_wait(&S.drain[0], 0); ++i) {
         }
-    } else if (warp == 9 || warp == 10) {
-        // ---- K rows (warp 9), V rows (warp 10) ----
+    } else if (warp == 11) {
+        // ---- O += P V: a warp of its own, because one thread that issued both products and kept both sides' barriers spent
+        // more time on those than the products take ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        constexpr uint32_t id_o = idesc_f16(kHalf, true, D);
+        const uint64_t v_desc = desc_v(smem_u32(Vs));
+        unsigned n = 0, vi = 0, vpar = 0;
+        bool ok = true;
+        while (ok && walk.next(x)) {
+            const bool pair = x.pair();
+            const unsigned ns = x.steps();
+            for (unsigned st = 0; st < ns; ++st, ++n) {
+                const int w = __shfl_sync(0xffffffffu, (int)(n & 1), 0), vs = __shfl_sync(0xffffffffu, (int)vi, 0);
+                const unsigned more = __shfl_sync(0xffffffffu, st >= 2 ? 1u : 0u, 0);  // adds to O
+                const bool last_v = !pair || (st & 1);
+                if ((!pair || !(st & 1)) && !(ok = attn_wait(&S.v_full[vs], vpar, &S, a.status, 534))) break;
+                if (!(ok = attn_wait(&S.p_ready[w], (n >> 1) & 1, &S, a.status, 535))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t vd = v_desc + (uint64_t)(vs * (C::kTileBytes >> 4));
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(tmem + C::kO + w * C::kOStep, tmem + C::kP + w * C::kPStep + 8 * k, vd + (uint64_t)(k * 2048 >> 4), id_o, k > 0 ? 1u : more);
+                    tc_commit(&S.pv_done[w]);
+                    if (last_v) tc_commit(&S.v_empty[vs]);
+                    if (st + 2 >= ns) tc_commit(&S.o_full[w]);
+                }
+                __syncwarp();
+                if (last_v && ++vi == C::kRing) vi = 0, vpar ^= 1;
+            }
+        }
+        if (elect_one()) tc_commit(&S.drain[1]);
+        __syncwarp();
+        for (uint32_t i = 0; i < kWaitPolls && !mbar_try_wait(&S.drain[1], 0); ++i) {
+        }
+    } else {
+        // ---- queries and K rows (warp 9), V rows (warp 10) ----
         // Where pages hold runs of 8 or more aligned rows, a lane copies a run as one box; else a lane gathers four rows. Rows
         // past the piece's last key are asked for behind the pool's end, which reads zeros: a probability of zero times
         // whatever a stale row holds would not be zero. So the run that the last key ends in is gathered row by row (V).
@@ -742,6 +842,37 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             };
             int y[4] = {0, 0, 0, 0};
             slots_of(x.t0, y);
+            for (int half = 0; !is_v && half < (x.pair() ? 2 : 1); ++half, ++q_count) {
+                const unsigned i = q_count % C::kQ;
+                if (!(ok = attn_wait(&S.q_empty[i], ((q_count / C::kQ) & 1) ^ 1, &S, a.status, 539))) break;
+                unsigned char* dst = Qs + i * C::kTileBytes;
+                const int ir = x.rb * 2 * kTile + half * kTile;  // the tile's first row in the item
+                if (a.q_box) {                                   // 128 / G whole tokens: one box a 64-wide column block
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&S.q_full[i], C::kTileBytes);
+#pragma unroll
+                        for (int c = 0; c < C::kAtoms; ++c)
+                            load_box3(dst + c * (kTile * 128), &maps.q, 64 * c, x.h * a.G, x.first + ir / a.G, &S.q_full[i]);
+                    }
+                    __syncwarp();
+                } else {
+#pragma unroll 1
+                    for (int r = lane; r < kTile; r += 32) {
+                        const bool valid = half * kTile + r < x.rows;
+                        const int tok = (ir + r) / a.G, head = x.h * a.G + ir + r - tok * a.G;
+                        const unsigned char* src =
+                            (const unsigned char*)a.q + (valid ? ((long long)(x.first + tok) * a.q_row + head * a.q_head) * 2 : 0);
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c)
+                            cp_async16(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + c * 16, valid);
+                    }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    fence_proxy_async_smem();
+                    mbar_arrive(&S.q_full[i]);
+                }
+            }
+            if (!ok) break;
             for (unsigned t = x.t0; t < x.t1; ++t) {
                 const unsigned i = issued % C::kRing;
                 if (!(ok = attn_wait(&empty[i], ((issued / C::kRing) & 1) ^ 1, &S, a.status, 537))) break;
@@ -772,44 +903,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 if (t + 1 < x.t1) slots_of(t + 1, y);
             }
         }
-    } else {
-        // ---- queries ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        unsigned q = 0;
-        bool ok = true;
-        while (ok && walk.next(x)) {
-            for (int half = 0; half < (x.pair() ? 2 : 1); ++half, ++q) {
-                const unsigned i = q % C::kQ;
-                if (!(ok = attn_wait(&S.q_empty[i], ((q / C::kQ) & 1) ^ 1, &S, a.status, 539))) break;
-                unsigned char* dst = Qs + i * C::kTileBytes;
-                const int ir = x.rb * 2 * kTile + half * kTile;  // the tile's first row in the item
-                if (a.q_box) {  // 128 / G whole tokens: one box a 64-wide column block
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&S.q_full[i], C::kTileBytes);
-#pragma unroll
-                        for (int c = 0; c < C::kAtoms; ++c)
-                            load_box3(dst + c * (kTile * 128), &maps.q, 64 * c, x.h * a.G, x.first + ir / a.G, &S.q_full[i]);
-                    }
-                    __syncwarp();
-                    ++q_boxes;
-                } else {
-#pragma unroll 1
-                    for (int r = lane; r < kTile; r += 32) {
-                        const bool valid = half * kTile + r < x.rows;
-                        const int tok = (ir + r) / a.G, head = x.h * a.G + ir + r - tok * a.G;
-                        const unsigned char* src =
-                            (const unsigned char*)a.q + (valid ? ((long long)(x.first + tok) * a.q_row + head * a.q_head) * 2 : 0);
-#pragma unroll
-                        for (int c = 0; c < D / 8; ++c)
-                            cp_async16(dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + c * 16, valid);
-                    }
-                    cp_async_commit();
-                    cp_async_wait<0>();
-                    fence_proxy_async_smem();
-                    mbar_arrive(&S.q_full[i]);
-                }
-            }
-        }
     }
     tc_fence_before();
     __syncthreads();
@@ -817,7 +910,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (warp >= 9 && *(volatile int*)&S.abort) {
+    if ((warp == 9 || warp == 10) && *(volatile int*)&S.abort) {
         // a role gave up: copies may still be on their way into this CTA's shared memory, so the last of each stage lands first
         auto landed = [&](uint64_t* full, unsigned stages, unsigned count) {
             for (unsigned i = 0; i < stages; ++i) {
@@ -826,8 +919,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 }
             }
         };
-        if (warp == 11) landed(S.q_full, C::kQ, q_boxes);
-        else landed(warp == 10 ? S.v_full : S.k_full, C::kRing, issued);
+        landed(warp == 10 ? S.v_full : S.k_full, C::kRing, issued);
+        if (warp == 9) landed(S.q_full, C::kQ, q_count);
     }
 }
 
@@ -851,17 +944,19 @@ template <int D, bool kHalf>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixAttnArgs a) {
     constexpr int kCols = D / 32;
     typedef typename Cols<kCols>::type V;
-    griddep_wait();
+    // Before its wait: everything that rests on the lengths alone (they are older than the first kernel).
     const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
-    const PlanHead h = *(const PlanHead*)a.ws;
-    const unsigned* cum = (const unsigned*)(a.ws + 256);
-    if (tok >= (int)h.tokens) return;
-    const int b = request_of(a, tok);
+    const bool inside = tok < a.rows;
+    const int b = request_of_warp(a, inside ? tok : 0, lane);
     const Req r = request(a, b);
-    const int j = tok - r.first;
-    if (j < 0 || j >= r.n) return;
-    const int kv = head / a.G, hg = head - kv * a.G;
+    const int j = tok - r.first, kv = head / a.G, hg = head - kv * a.G;
+    const int own_rows = r.n * a.G, gr = j * a.G + hg, rb = gr / (2 * kTile);
+    griddep_wait();
+    const unsigned* cum = (const unsigned*)(a.ws + 256);
+    const PlanHead h = *(const PlanHead*)a.ws;
+    const unsigned cum_step = cum[b], cum_item = cum[a.batch + b];
+    if (!inside || tok >= (int)h.tokens || j < 0 || j >= r.n) return;
 
     float M = -INFINITY, Ls = 0.f, o[kCols];
 #pragma unroll
@@ -871,7 +966,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixAttnArgs 
     auto item = [&](unsigned first, unsigned tiles, int rows, int index, int rr, const unsigned char* base, int R) {
         const int sh = rows > kTile ? 1 : 0;
         const unsigned len = (tiles << sh) + kItemSteps;
-        const int c0 = cta_of(first, h.total, a.ctas), c1 = cta_of(first + len - 1, h.total, a.ctas);
+        const int c0 = cta_of(first, h.total), c1 = cta_of(first + len - 1, h.total);
         const long long part = part_bytes(R, D);
         const int row = rr & (kTile - 1), half = rr >> 7;
         const int lanes = sh ? 32 : 16;  // CTAs looked up at once
@@ -880,7 +975,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixAttnArgs 
             float m = -INFINITY, l = 0.f;
             const float* src = nullptr;
             if (c <= c1) {
-                const unsigned lo = max(range_lo(h.total, c, a.ctas), first), hi = min(range_lo(h.total, c + 1, a.ctas), first + len);
+                const unsigned lo = max(range_lo(h.total, c), first), hi = min(range_lo(h.total, c + 1), first + len);
                 unsigned t0 = 0, t1 = 0;
                 if (hi > lo) tiles_of(lo - first, hi - first, sh, t0, t1);
                 if (t1 > t0 + (sh ? 0 : s)) {
@@ -889,47 +984,51 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixAttnArgs 
                     l = src[(long long)R * D + R + row];
                 }
             }
-            const float mn = fmaxf(M, warp_max(m));
-            const float f = M == mn ? 1.f : ex2(M - mn);                      // of what is there
-            const float g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
-            M = mn;
-            Ls = Ls * f + warp_sum(l * g);
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) o[i] *= f;
-            unsigned there = __ballot_sync(0xffffffffu, l != 0.f);
+            // O of up to 16 pieces is asked for before the first m and l are looked at
+            unsigned there = __ballot_sync(0xffffffffu, src != nullptr);
+            float mn = M, f = 1.f, g = 0.f;
+            bool weighed = false;
             while (there != 0u) {
-                V v[4];
-                float w[4];
+                V v[16];
+                int from[16];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int from = there != 0u ? __ffs(there) - 1 : 0;
-                    const bool on = there != 0u;
+                for (int i = 0; i < 16; ++i) {
+                    from[i] = there != 0u ? __ffs(there) - 1 : -1;
                     there &= there - 1;
-                    const float* at = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, from);
-                    w[i] = __shfl_sync(0xffffffffu, g, from);
-                    if (on) v[i] = *(const V*)(at + ((long long)(lane * kCols >> 2) * R + row) * 4 + (lane * kCols & 3));
-                    else w[i] = 0.f, v[i] = V();
+                    const float* at = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, from[i] < 0 ? 0 : from[i]);
+                    if (from[i] >= 0) v[i] = *(const V*)(at + ((long long)(lane * kCols >> 2) * R + row) * 4 + (lane * kCols & 3));
+                }
+                if (!weighed) {
+                    weighed = true;
+                    mn = fmaxf(M, warp_max(m));
+                    f = M == mn ? 1.f : ex2(M - mn);                      // of what is there
+                    g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
+                    M = mn;
+                    Ls = Ls * f + warp_sum(l * g);
+#pragma unroll
+                    for (int i = 0; i < kCols; ++i) o[i] *= f;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float* e = (const float*)&v[i];
+                for (int i = 0; i < 16; ++i) {
+                    const float w = __shfl_sync(0xffffffffu, g, from[i] < 0 ? 0 : from[i]);
+                    if (from[i] >= 0) {
+                        const float* e = (const float*)&v[i];
 #pragma unroll
-                    for (int k = 0; k < kCols; ++k) o[k] += e[k] * w[i];
+                        for (int k = 0; k < kCols; ++k) o[k] = w == 0.f ? o[k] : o[k] + e[k] * w;
+                    }
                 }
             }
         }
     };
     if (h.tiles > 0) {
-        const int total = (int)h.tokens * a.G, gr = tok * a.G + hg, rb = gr / (2 * kTile), blocks = row_blocks(total);
-        item(kv * h.per_head + rb * (2 * h.tiles + kItemSteps), h.tiles, min(2 * kTile, total - rb * 2 * kTile), kv * blocks + rb, gr - rb * 2 * kTile,
-             a.ws + a.ws_prefix, kTile);
+        const int total = (int)h.tokens * a.G, pr = tok * a.G + hg, pb = pr / (2 * kTile);
+        item(kv * h.per_head + pb * (2 * h.tiles + kItemSteps), h.tiles, min(2 * kTile, total - pb * 2 * kTile), kv * row_blocks(total) + pb,
+             pr - pb * 2 * kTile, a.ws + a.ws_prefix, kTile);
     }
     const unsigned tiles = own_tiles(a, r, (int)h.prefix);
-    if (tiles > 0) {
-        const int total = r.n * a.G, gr = j * a.G + hg, rb = gr / (2 * kTile), blocks = row_blocks(total);
-        item(cum[b] + kv * head_steps(tiles, total) + rb * (2 * tiles + kItemSteps), tiles, min(2 * kTile, total - rb * 2 * kTile),
-             (int)cum[a.batch + b] + kv * blocks + rb, gr - rb * 2 * kTile, a.ws + a.ws_suffix, a.suffix_rows);
-    }
+    if (tiles > 0)
+        item(cum_step + kv * head_steps(tiles, own_rows) + rb * (2 * tiles + kItemSteps), tiles, min(2 * kTile, own_rows - rb * 2 * kTile),
+             (int)cum_item + kv * row_blocks(own_rows) + rb, gr - rb * 2 * kTile, a.ws + a.ws_suffix, a.suffix_rows);
     const float inv = Ls == 0.f ? 0.f : 1.f / Ls;  // a row that saw no key is zero
     uint32_t w[kCols / 2];
 #pragma unroll
@@ -946,7 +1045,7 @@ static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const PrefixAttnMaps
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.ctas);
+    cfg.gridDim = dim3(kCtas);
     cfg.blockDim = dim3(kAttnThreads);
     cfg.dynamicSmemBytes = Cfg<D>::kSmem;
     cfg.stream = s;

@@ -1083,7 +1083,7 @@ int mk_launch_info(const MkLaunch* launch, MkLaunchInfo* out) {
         out->smem = L->op_kind[0] == OP_GEMM_BF16 ? (int64_t)gemm_smem(L->op_gemm, false) : 0;
         if (L->op_kind[0] == OP_PREFIX_ATTN) {
             out->kernels = 2;
-            out->grid = L->pattn.ctas;
+            out->grid = kAttnCtas;
         }
         out->param_bytes = (int64_t)sizeof(MkLaunch);
         return 0;

@@ -3,8 +3,8 @@
 
 A step runs ``BlockTables`` (pages, slots and positions of its new tokens), ``Rotary`` per layer (rotation of q and k by the
 rows of a ``RopeTable``, append of k and v at the slots) and ``PrefixAttention`` per layer (the new rows over the pool, the
-prefix that all requests share visited once). Each class owns its outputs and scratch, binds once and launches on a stream
-(graph-capturable: lengths are read on the device). A bound object may not overlap itself on two streams.
+prefix that all requests share visited once). Each class owns its outputs and scratch, binds once, and ``launch(stream, pdl)``
+enqueues it (graph-capturable: lengths are read on the device). A bound object may not overlap itself on two streams.
 
 ``status`` of each (i32 [16]) stays 0 until a launch leaves something out; ``include/mk_abi.h`` lists what.
 """
@@ -94,10 +94,7 @@ class BlockTables:
             free_words=free_words, page_size=page_size, batch=batch, rows=rows, block_table=self.block_table, slots=self.slots,
             positions=self.positions, cu_rows=self.cu_rows, kv_lens=self.kv_lens, ticket=self.ticket, status=self.status,
         )  # fmt: skip
-        self.launch_record = lib.bind("mk_block_tables_bind", module, self.bind)
-
-    def launch(self, stream: int, pdl: bool = False) -> None:
-        self.launch_record(stream, pdl)
+        self.launch = lib.bind("mk_block_tables_bind", module, self.bind)
 
 
 class RopeTable:
@@ -120,10 +117,7 @@ class RopeTable:
         fields.update({k: float(v) for k, v in sc.items()})
         self.bind = host.make("MkRopeTableBind", out=self.cos_sin, rows=rows, first=first, rot=rot, theta=float(theta),
                               kind=ROPE_KINDS[kind], **fields)  # fmt: skip
-        self.launch_record = lib.bind("mk_rope_table_bind", module, self.bind)
-
-    def launch(self, stream: int, pdl: bool = False) -> None:
-        self.launch_record(stream, pdl)
+        self.launch = lib.bind("mk_rope_table_bind", module, self.bind)
 
 
 class Rotary:
@@ -172,10 +166,7 @@ class Rotary:
             rows=rows, q_heads=qh, kv_heads=kvh, head_dim=dim, rot=cos_sin_cache.shape[1], interleaved=int(interleaved),
             inverse=int(inverse), fp16=int(dt == torch.float16), status=self.status, **st,
         )  # fmt: skip
-        self.launch_record = lib.bind("mk_rotary_bind", module, self.bind)
-
-    def launch(self, stream: int, pdl: bool = False) -> None:
-        self.launch_record(stream, pdl)
+        self.launch = lib.bind("mk_rotary_bind", module, self.bind)
 
 
 class PrefixAttention:
@@ -221,7 +212,4 @@ class PrefixAttention:
         self.ws = torch.empty(self.consts.ws_bytes, dtype=torch.uint8, device=dev)
         fields.update(ws=self.ws, ws_bytes=self.consts.ws_bytes)
         self.bind = host.make("MkPrefixAttnBind", **fields)
-        self.launch_record = lib.bind("mk_prefix_attn_bind", module, self.bind)
-
-    def launch(self, stream: int, pdl: bool = False) -> None:
-        self.launch_record(stream, pdl)
+        self.launch = lib.bind("mk_prefix_attn_bind", module, self.bind)
