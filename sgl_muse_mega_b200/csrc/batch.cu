@@ -206,9 +206,11 @@ __global__ void __launch_bounds__(128) rope_table_kernel(const RopeTableArgs a) 
     const long long id = (long long)blockIdx.x * 128 + threadIdx.x;
     const int f = (int)(id % groups) * 4;
     const long long r0 = id / groups * kRows;
-    double c[4], s[4];
+    double c[4], s[4], cs[4], sn[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        cs[j] = a.step[f + j].x;
+        sn[j] = a.step[f + j].y;
         const double t = (double)(a.first + r0) * a.turns[f + j];
         sincospi(2.0 * (t - rint(t)), &s[j], &c[j]);
         c[j] *= a.mult;
@@ -224,9 +226,9 @@ __global__ void __launch_bounds__(128) rope_table_kernel(const RopeTableArgs a) 
         out += a.rot;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const double cs = a.step[f + j].x, sn = a.step[f + j].y, x = c[j];
-            c[j] = x * cs - s[j] * sn;
-            s[j] = s[j] * cs + x * sn;
+            const double x = c[j];
+            c[j] = x * cs[j] - s[j] * sn[j];
+            s[j] = s[j] * cs[j] + x * sn[j];
         }
     }
 }
@@ -267,58 +269,65 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     typedef Pair<T> P2;
     typedef typename P2::type T2;
     griddep_wait();
+    // Nothing waits for anything it does not need: the row's words and the first heads are asked for together, the table row
+    // follows the position, the checks come behind all loads (the row lies inside the tensors whether it is live or not).
     const int r = blockIdx.x;
-    if (a.n_rows != nullptr && r >= *a.n_rows) return;
+    const int n_rows = a.n_rows != nullptr ? *a.n_rows : a.rows;
     long long pos = a.positions[r];
-    if (pos < 0 || pos >= a.cos_rows) {
-        if (threadIdx.x == 0) batch_status(a.status, 4, 510, (int)pos, (int)min(a.cos_rows, 0x7fffffffll));
-        pos = 0;
-    }
-    long long slot = -1;
-    if (a.k_cache != nullptr) {
-        slot = a.slots[r];
-        if (slot >= a.kv_rows) {
-            if (threadIdx.x == 0) batch_status(a.status, 4, 511, (int)min(slot, 0x7fffffffll), (int)min(a.kv_rows, 0x7fffffffll));
-            slot = -1;
-        }
-    }
+    long long slot = a.k_cache != nullptr ? a.slots[r] : -1;
     const T* qr = (const T*)a.q + r * a.q_row;
     const T* kr = (const T*)a.k + r * a.k_row;
     T* qo = (T*)a.q_out + r * a.qo_row;
     T* ko = a.k_out != nullptr ? (T*)a.k_out + r * a.ko_row : nullptr;
-    T* kc = slot >= 0 ? (T*)a.k_cache + slot * a.kc_row : nullptr;
-    const float* tab = a.cos_sin + pos * a.rot;
     const int half = a.rot / 2;
     // pieces of a head: the rotated ones (a piece holds N pairs in the half layout, N / 2 in the interleaved one), then the rest
     const int turn = kInter ? a.rot / N : half / N, pieces = turn + (a.dim - a.rot) / N;
     const int step = blockDim.x / pieces, c = threadIdx.x % pieces;
-    if ((int)threadIdx.x < step * pieces) {
-        constexpr int kHeads = 3;  // heads in flight a thread: their loads go out before the table row is needed
-        const bool turned = c < turn;
-        const int at = turned ? c * N : a.rot + (c - turn) * N;
+    constexpr int kHeads = 3;  // heads in flight a thread
+    const bool mine = (int)threadIdx.x < step * pieces, turned = c < turn;
+    const int at = turned ? c * N : a.rot + (c - turn) * N;
+    int h0 = mine ? (int)threadIdx.x / pieces : a.qh + a.kvh;
+    W w0[kHeads], w1[kHeads];
+    auto load_heads = [&]() {
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const int hh = h0 + i * step;
+            if (hh < a.qh + a.kvh) {
+                const T* src = hh < a.qh ? qr + hh * a.q_head : kr + (hh - a.qh) * a.k_head;
+                w0[i] = *(const W*)(src + at);
+                if (!kInter && turned) w1[i] = *(const W*)(src + half + at);
+            }
+        }
+    };
+    load_heads();
+    // v: from the block's last thread backwards, as the first threads have the heads' remainder
+    const T* vr = (const T*)a.v + r * a.v_row;
+    const int vp = a.dim / 8, v0 = blockDim.x - 1 - threadIdx.x;
+    uint4 vw = make_uint4(0, 0, 0, 0);
+    if (a.v != nullptr && v0 < a.kvh * vp) vw = *(const uint4*)(vr + v0 / vp * a.v_head + v0 % vp * 8);
+    if (r >= n_rows) return;
+    if (pos < 0 || pos >= a.cos_rows) {
+        if (threadIdx.x == 0) batch_status(a.status, 4, 510, (int)pos, (int)min(a.cos_rows, 0x7fffffffll));
+        pos = 0;
+    }
+    if (slot >= a.kv_rows && a.k_cache != nullptr) {
+        if (threadIdx.x == 0) batch_status(a.status, 4, 511, (int)min(slot, 0x7fffffffll), (int)min(a.kv_rows, 0x7fffffffll));
+        slot = -1;
+    }
+    T* kc = slot >= 0 ? (T*)a.k_cache + slot * a.kc_row : nullptr;
+    const float* tab = a.cos_sin + pos * a.rot;
+    if (mine) {
         float cs[N], sn[N];
-        bool have = false;
-        for (int h0 = threadIdx.x / pieces; h0 < a.qh + a.kvh; h0 += kHeads * step) {
-            W w0[kHeads], w1[kHeads];
+        if (turned) {
+            constexpr int n = kInter ? N / 2 : N;
 #pragma unroll
-            for (int i = 0; i < kHeads; ++i) {
-                const int hh = h0 + i * step;
-                if (hh < a.qh + a.kvh) {
-                    const T* src = hh < a.qh ? qr + hh * a.q_head : kr + (hh - a.qh) * a.k_head;
-                    w0[i] = *(const W*)(src + at);
-                    if (!kInter && turned) w1[i] = *(const W*)(src + half + at);
-                }
+            for (int j = 0; j < n; j += 2) {
+                const float2 x = *(const float2*)(tab + c * n + j), y = *(const float2*)(tab + half + c * n + j);
+                cs[j] = x.x, cs[j + 1] = x.y;
+                sn[j] = a.inverse ? -y.x : y.x, sn[j + 1] = a.inverse ? -y.y : y.y;
             }
-            if (!have && turned) {
-                constexpr int n = kInter ? N / 2 : N;
-#pragma unroll
-                for (int j = 0; j < n; j += 2) {
-                    const float2 x = *(const float2*)(tab + c * n + j), y = *(const float2*)(tab + half + c * n + j);
-                    cs[j] = x.x, cs[j + 1] = x.y;
-                    sn[j] = a.inverse ? -y.x : y.x, sn[j + 1] = a.inverse ? -y.y : y.y;
-                }
-            }
-            have = true;
+        }
+        while (true) {
 #pragma unroll
             for (int i = 0; i < kHeads; ++i) {
                 const int hh = h0 + i * step;
@@ -353,16 +362,16 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
                 }
                 put(at, w0[i]);
             }
+            h0 += kHeads * step;
+            if (h0 >= a.qh + a.kvh) break;
+            load_heads();
         }
     }
     if (a.v != nullptr && slot >= 0) {
-        const T* vr = (const T*)a.v + r * a.v_row;
         T* vc = (T*)a.v_cache + slot * a.vc_row;
-        const int vp = a.dim / 8;
-        // from the block's last thread backwards: the first threads have had the heads' remainder
-        for (int i = blockDim.x - 1 - threadIdx.x; i < a.kvh * vp; i += blockDim.x) {
+        for (int i = v0; i < a.kvh * vp; i += blockDim.x) {
             const int h = i / vp, d = (i - h * vp) * 8;
-            *(uint4*)(vc + h * a.vc_head + d) = *(const uint4*)(vr + h * a.v_head + d);
+            *(uint4*)(vc + h * a.vc_head + d) = i == v0 ? vw : *(const uint4*)(vr + h * a.v_head + d);
         }
     }
 }
