@@ -219,9 +219,11 @@ __device__ __forceinline__ Plan make_plan(const PrefixAttnArgs& a, const Lens& l
 constexpr unsigned kCtas = kAttnCtas;
 __device__ __forceinline__ unsigned range_lo(unsigned total, unsigned c) {  // first step of CTA c's range: floor(total c / kCtas)
     const unsigned q = total / kCtas;
+    if (q == 0) return min(c, total);  // fewer steps than CTAs: one each
     return q * c + (total - q * kCtas) * c / kCtas;
 }
 __device__ __forceinline__ int cta_of(unsigned step, unsigned total) {  // whose range holds the step
+    if (total < kCtas) return (int)step;
     if (total < (1u << 24)) return (int)(((step + 1) * kCtas - 1) / total);  // kCtas < 2^8
     return (int)((((unsigned long long)step + 1) * kCtas - 1) / total);
 }
@@ -532,7 +534,7 @@ __device__ __forceinline__ void row_keys(const PrefixAttnArgs& a, const Plan& p,
 
 template <int D, bool kHalf>
 __global__ void __launch_bounds__(kAttnThreads, 1)
-    prefix_attn_kernel(const PrefixAttnArgs a, const __grid_constant__ PrefixAttnMaps maps) {
+    prefix_attn_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ PrefixAttnMaps maps) {
     typedef Cfg<D> C;
     extern __shared__ unsigned char raw[];
     __shared__ Bars S;
@@ -924,118 +926,123 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
 }
 
-template <int N>
-struct Cols;
-template <>
-struct Cols<2> {
-    typedef float2 type;
-};
-template <>
-struct Cols<4> {
-    typedef float4 type;
-};
-
 // ---- merge --------------------------------------------------------------------------------------------------------------
-// Row r of an item's pieces: M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L. A warp takes one row: its lanes
-// look up a piece each (the CTA's range, its slot, m and l; all loads of 32 pieces at once), then walk the pieces
-// together, D / 32 output columns a lane. The eight rows of a block are neighbours (heads of one token mostly), whose O
-// values share 128-byte lines.
+// out = sum O_i 2^(m_i - M) / L over the pieces of the row's prefix item and own item, M = max m_i, L = sum l_i 2^(m_i - M). A
+// warp takes one row. Its lanes look up a candidate piece each (a CTA of the item's range, a part of its slot): which slot, m
+// and l, all requested at once; then D / 4 lanes read a piece's O (a float4 each), eight loads in flight, in the order of the
+// candidates. What rests on the lengths alone is done before the wait for the first kernel. The time is the chain of
+// three round trips to L2 (plan, m and l, O) behind that kernel's end.
 template <int D, bool kHalf>
-__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixAttnArgs a) {
-    constexpr int kCols = D / 32;
-    typedef typename Cols<kCols>::type V;
-    // Before its wait: everything that rests on the lengths alone (they are older than the first kernel).
+__global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant__ PrefixAttnArgs a) {
+    constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;  // lanes of a piece, pieces read side by side
     const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
     const bool inside = tok < a.rows;
     const int b = request_of_warp(a, inside ? tok : 0, lane);
     const Req r = request(a, b);
     const int j = tok - r.first, kv = head / a.G, hg = head - kv * a.G;
-    const int own_rows = r.n * a.G, gr = j * a.G + hg, rb = gr / (2 * kTile);
     griddep_wait();
     const unsigned* cum = (const unsigned*)(a.ws + 256);
     const PlanHead h = *(const PlanHead*)a.ws;
     const unsigned cum_step = cum[b], cum_item = cum[a.batch + b];
     if (!inside || tok >= (int)h.tokens || j < 0 || j >= r.n) return;
 
-    float M = -INFINITY, Ls = 0.f, o[kCols];
+    // the prefix item and the own item: first step, steps, first CTA and number of candidates, slot of CTA 0, place of the row
+    struct Item {
+        unsigned first, len;
+        int sh, c0, n, index, R, row, half;
+    };
+    const bool alone = h.total < kCtas;  // one step a CTA: no second parts
+    auto item = [&](unsigned tiles, int rows, int gr, unsigned first, int index, int R) {
+        Item e;
+        const int block = gr / (2 * kTile), rr = gr - block * 2 * kTile, left = min(2 * kTile, rows - block * 2 * kTile);
+        e.sh = left > kTile ? 1 : 0;
+        e.first = first + kv * head_steps(tiles, rows) + block * (2 * tiles + kItemSteps);
+        e.len = (tiles << e.sh) + kItemSteps;
+        e.index = index + kv * row_blocks(rows) + block;
+        e.R = R;
+        e.row = rr & (kTile - 1);
+        e.half = rr >> 7;
+        e.c0 = tiles > 0 ? cta_of(e.first + kItemSteps, h.total) : 0;
+        e.n = tiles > 0 ? (cta_of(e.first + e.len - 1, h.total) - e.c0 + 1) << (e.sh || alone ? 0 : 1) : 0;
+        return e;
+    };
+    const Item pre = item(h.tiles, (int)h.tokens * a.G, tok * a.G + hg, 0u, 0, kTile);
+    const Item ind = item(own_tiles(a, r, (int)h.prefix), r.n * a.G, j * a.G + hg, cum_step, (int)cum_item, a.suffix_rows);
+    float M = -INFINITY, Ls = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < pre.n + ind.n; k0 += 32) {
+        const int k = k0 + lane;
+        const bool own = k >= pre.n;
+        const int q = own ? k - pre.n : k, n = own ? ind.n : pre.n, sh = own ? ind.sh : pre.sh, R = own ? ind.R : pre.R, row = own ? ind.row : pre.row;
+        const bool one = sh != 0 || alone;
+        const int c = (own ? ind.c0 : pre.c0) + (one ? q : q >> 1), s = sh != 0 ? (own ? ind.half : pre.half) : one ? 0 : q & 1;
+        const unsigned first = own ? ind.first : pre.first, len = own ? ind.len : pre.len;
+        bool on = false;
+        if (q < n) {
+            const unsigned lo = max(range_lo(h.total, c), first), hi = min(range_lo(h.total, c + 1), first + len);
+            unsigned t0 = 0, t1 = 0;
+            if (hi > lo) tiles_of(lo - first, hi - first, sh, t0, t1);
+            on = t1 > t0 + (sh != 0 ? 0 : s);
+        }
+        const float4* src =
+            (const float4*)(a.ws + (own ? a.ws_suffix : a.ws_prefix) + ((long long)((own ? ind.index : pre.index) + c) * 2 + s) * part_bytes(R, D)) + row;
+        float m = -INFINITY, l = 0.f;
+        if (on) {
+            const float* ml = (const float*)(src - row + R * (D / 4)) + row;
+            m = ml[0];
+            l = ml[R];
+        }
+        unsigned there = __ballot_sync(0xffffffffu, on);
+        const unsigned owned = __ballot_sync(0xffffffffu, own);
+        bool weighed = false;
+        float g = 0.f;
+        while (there != 0u) {  // O is asked for before m and l are looked at
+            constexpr int kAhead = 8;
+            float4 v[kAhead];
+            int from[kAhead];
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) o[i] = 0.f;
-    // all pieces of the item whose first step is `first`, for its block row `rr`: two candidates a CTA (its parts), one
-    // candidate a lane
-    auto item = [&](unsigned first, unsigned tiles, int rows, int index, int rr, const unsigned char* base, int R) {
-        const int sh = rows > kTile ? 1 : 0;
-        const unsigned len = (tiles << sh) + kItemSteps;
-        const int c0 = cta_of(first, h.total), c1 = cta_of(first + len - 1, h.total);
-        const long long part = part_bytes(R, D);
-        const int row = rr & (kTile - 1), half = rr >> 7;
-        const int lanes = sh ? 32 : 16;  // CTAs looked up at once
-        for (int cb = c0; cb <= c1; cb += lanes) {
-            const int c = cb + (sh ? lane : lane >> 1), s = sh ? half : lane & 1;
-            float m = -INFINITY, l = 0.f;
-            const float* src = nullptr;
-            if (c <= c1) {
-                const unsigned lo = max(range_lo(h.total, c), first), hi = min(range_lo(h.total, c + 1), first + len);
-                unsigned t0 = 0, t1 = 0;
-                if (hi > lo) tiles_of(lo - first, hi - first, sh, t0, t1);
-                if (t1 > t0 + (sh ? 0 : s)) {
-                    src = (const float*)(base + ((long long)(index + c) * 2 + s) * part);
-                    m = src[(long long)R * D + row];
-                    l = src[(long long)R * D + R + row];
-                }
-            }
-            // O of up to 16 pieces is asked for before the first m and l are looked at
-            unsigned there = __ballot_sync(0xffffffffu, src != nullptr);
-            float mn = M, f = 1.f, g = 0.f;
-            bool weighed = false;
-            while (there != 0u) {
-                V v[16];
-                int from[16];
+            for (int i = 0; i < kAhead; ++i) {
+                from[i] = 32;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    from[i] = there != 0u ? __ffs(there) - 1 : -1;
+                for (int y = 0; y < kAtOnce; ++y) {
+                    const int f = there != 0u ? __ffs(there) - 1 : 32;
                     there &= there - 1;
-                    const float* at = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, from[i] < 0 ? 0 : from[i]);
-                    if (from[i] >= 0) v[i] = *(const V*)(at + ((long long)(lane * kCols >> 2) * R + row) * 4 + (lane * kCols & 3));
+                    if (lane / kLanes == y) from[i] = f;
                 }
-                if (!weighed) {
-                    weighed = true;
-                    mn = fmaxf(M, warp_max(m));
-                    f = M == mn ? 1.f : ex2(M - mn);                      // of what is there
-                    g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
-                    M = mn;
-                    Ls = Ls * f + warp_sum(l * g);
+                const float4* p = (const float4*)__shfl_sync(0xffffffffu, (unsigned long long)src, from[i] & 31);
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (from[i] < 32) v[i] = p[(lane % kLanes) * ((owned >> from[i]) & 1u ? a.suffix_rows : kTile)];
+            }
+            if (!weighed) {
+                weighed = true;
+                const float mn = fmaxf(M, warp_max(m));
+                const float f = M == mn ? 1.f : ex2(M - mn);   // of what is there
+                g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
+                M = mn;
+                Ls = Ls * f + warp_sum(l * g);
 #pragma unroll
-                    for (int i = 0; i < kCols; ++i) o[i] *= f;
-                }
+                for (int i = 0; i < 4; ++i) o[i] *= f;
+            }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float w = __shfl_sync(0xffffffffu, g, from[i] < 0 ? 0 : from[i]);
-                    if (from[i] >= 0) {
-                        const float* e = (const float*)&v[i];
-#pragma unroll
-                        for (int k = 0; k < kCols; ++k) o[k] = w == 0.f ? o[k] : o[k] + e[k] * w;
-                    }
+            for (int i = 0; i < kAhead; ++i) {
+                const float w = __shfl_sync(0xffffffffu, g, from[i] & 31);
+                if (from[i] < 32 && w != 0.f) {
+                    o[0] += v[i].x * w;
+                    o[1] += v[i].y * w;
+                    o[2] += v[i].z * w;
+                    o[3] += v[i].w * w;
                 }
             }
         }
-    };
-    if (h.tiles > 0) {
-        const int total = (int)h.tokens * a.G, pr = tok * a.G + hg, pb = pr / (2 * kTile);
-        item(kv * h.per_head + pb * (2 * h.tiles + kItemSteps), h.tiles, min(2 * kTile, total - pb * 2 * kTile), kv * row_blocks(total) + pb,
-             pr - pb * 2 * kTile, a.ws + a.ws_prefix, kTile);
     }
-    const unsigned tiles = own_tiles(a, r, (int)h.prefix);
-    if (tiles > 0)
-        item(cum_step + kv * head_steps(tiles, own_rows) + rb * (2 * tiles + kItemSteps), tiles, min(2 * kTile, own_rows - rb * 2 * kTile),
-             (int)cum_item + kv * row_blocks(own_rows) + rb, gr - rb * 2 * kTile, a.ws + a.ws_suffix, a.suffix_rows);
-    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;  // a row that saw no key is zero
-    uint32_t w[kCols / 2];
+    if (kAtOnce == 2) {
 #pragma unroll
-    for (int i = 0; i < kCols / 2; ++i) w[i] = pack2<kHalf>(o[2 * i] * inv, o[2 * i + 1] * inv);
-    uint32_t* out = (uint32_t*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * kCols) * 2);
-    if (kCols == 4) *(uint2*)out = make_uint2(w[0], w[kCols / 2 - 1]);
-    else *out = w[0];
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 16);
+    }
+    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;  // a row that saw no key is zero
+    if (lane < kLanes)
+        *(uint2*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * 4) * 2) =
+            make_uint2(pack2<kHalf>(o[0] * inv, o[1] * inv), pack2<kHalf>(o[2] * inv, o[3] * inv));
     if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + log2f(Ls)) * kLn2;
 }
 
