@@ -426,6 +426,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, float* r) {
           "=r"(u[31])
         : "r"(t));
 }
+// waits for this thread's loads; the registers pass through it, so that nothing that uses them moves in front
+__device__ __forceinline__ void tmem_arrived32(float* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]),
+                   "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]),
+                   "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]),
+                   "+f"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -452,26 +462,23 @@ __device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either i
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
     return r;
 }
-// 2^x for two x >= -126 on the FMA pipe: x = k + f with k the nearest whole number, 2^f on [-1/2, 1/2] by the polynomial of
-// degree 4 with the least relative error (2.7e-6; exchange algorithm), k added to the exponent. The special-function unit
-// gives 16 results a clock and SM, which bounds the softmax of 64-wide heads; kPolyOf8 of 8 results come from here.
+// 2^x for two x on the FMA pipe: x = k + f with k the nearest whole number, 2^f on [-1/2, 1/2] by the polynomial of degree 4 with
+// p(0) = 1 and the least relative error (2.9e-6; a linear program), k added to the exponent. x is kept at or above -127, where
+// the sum of exponents is exactly 0: a masked score (-inf) gives an exact zero. The special-function unit yields 16 results a
+// clock and SM, which would bound the softmax of 64-wide heads; kPolyOf8 of 8 results come from here instead.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
     const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
+    x.x = fmaxf(x.x, -127.f);
+    x.y = fmaxf(x.y, -127.f);
     const float2 r = add2(x, magic);  // k in the low bits
     const float2 f = fma2(add2(r, back), make_float2(-1.f, -1.f), x);
-    float2 p = fma2(f, make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f), make_float2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    p = fma2(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    p = fma2(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    p = fma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    float2 p = fma2(f, make_float2(0x1.3a007ap-7f, 0x1.3a007ap-7f), make_float2(0x1.c9fd1ep-5f, 0x1.c9fd1ep-5f));
+    p = fma2(p, f, make_float2(0x1.ec0382p-3f, 0x1.ec0382p-3f));
+    p = fma2(p, f, make_float2(0x1.62e12ap-1f, 0x1.62e12ap-1f));
+    p = fma2(p, f, make_float2(1.f, 1.f));
     return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
 constexpr int kPolyOf8 = 3;
-template <int N>
-struct Int {
-    static constexpr int value = N;
-};
 
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -621,33 +628,37 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 if (!(ok = attn_wait(&S.s_full[wg], s_par, &S, a.status, 530))) break;
                 s_par ^= 1;
                 tc_fence_after();
-                float s[128];
                 if (busy) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_ld32(tS + 32 * i, s + 32 * i);
-                    tmem_ld_wait();
-                }
-                if (!C::kAlias) {  // the scores are in registers: the tensor core may write the next ones
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&S.s_free[wg]);
-                }
-                if (busy) {
+                    // Two passes over the scores, 32 columns at a time from tensor memory (the next 32 on their way): the
+                    // maximum, then the probabilities. Loops of few instructions: a step's code unrolled over 128 columns
+                    // ran at the pace of instruction fetch where it ran once or twice (a launch of few steps: 4 us a step).
                     const bool whole = __all_sync(0xffffffffu, (lo <= kb && hi >= kb + kTile) || rr >= x.rows);
-                    if (!whole) {
-                        const int c0 = lo - kb, c1 = hi - kb;
+                    float s0[32], s1[32];
+                    auto hide = [&](float* s, int col) {
+                        const int c0 = lo - kb - col, c1 = hi - kb - col;
 #pragma unroll
-                        for (int i = 0; i < 128; ++i) s[i] = i >= c0 && i < c1 ? s[i] : -INFINITY;
+                        for (int i = 0; i < 32; ++i) s[i] = i >= c0 && i < c1 ? s[i] : -INFINITY;
+                    };
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    auto highest = [&](float* s, int col) {
+                        if (!whole) hide(s, col);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            mx[0] = max_nan(mx[0], max_nan(s[i], s[i + 1]));
+                            mx[1] = max_nan(mx[1], max_nan(s[i + 2], s[i + 3]));
+                        }
+                    };
+                    tmem_ld32(tS, s0);
+#pragma unroll 1
+                    for (int i = 0; i < 128; i += 64) {
+                        tmem_arrived32(s0);
+                        tmem_ld32(tS + i + 32, s1);
+                        highest(s0, i);
+                        tmem_arrived32(s1);
+                        tmem_ld32(tS + ((i + 64) & 127), s0);  // at the end: the first columns again, for the second pass
+                        highest(s1, i + 32);
                     }
-                    float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                    for (int i = 4; i < 124; i += 8) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) mx[j] = max_nan(mx[j], max_nan(s[i + j], s[i + 4 + j]));
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mx[j] = max_nan(mx[j], s[124 + j]);
-                    const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.scale_log2;
+                    const float top = max_nan(mx[0], mx[1]) * a.scale_log2;
                     if (!(top < INFINITY)) l = NAN;  // a score that is NaN or +inf: so is the row's softmax
                     // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
                     // P's type and the f32 sums carry without loss), so O is seldom rescaled.
@@ -660,40 +671,55 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     if (!C::kAlias && !(ok = attn_wait(&S.pv_done[wg], pv_par, &S, a.status, 540))) break;
                     if (any && st != sub) {
                         tc_fence_after();
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i) {
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 16) {
                             uint32_t o[16];
-                            tmem_ld16(tO + 16 * i, o);
+                            tmem_ld16(tO + i, o);
                             tmem_ld_wait();
 #pragma unroll
                             for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tmem_st16(tO + 16 * i, o);
+                            tmem_st16(tO + i, o);
                         }
                     }
                     const float ms = m == -INFINITY ? 0.f : m;
                     const float2 neg = make_float2(-ms, -ms);
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    auto probabilities = [&](auto poly) {
+                    auto probabilities = [&](float* s, int col) {
+                        if (!whole) hide(s, col);
+                        uint32_t u[16];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t u[16];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                float2 e = fma2(make_float2(s[32 * i + 2 * j], s[32 * i + 2 * j + 1]), scale2, neg);
-                                if (j % 8 < decltype(poly)::value) e = exp2_poly(e);
-                                else e = make_float2(ex2(e.x), ex2(e.y));
-                                sum[j & 1] = add2(sum[j & 1], e);
-                                u[j] = pack2<kHalf>(e.x, e.y);
-                            }
-                            tmem_st16(tP + 16 * i, u);
+                        for (int j = 0; j < 16; ++j) {
+                            float2 e = fma2(make_float2(s[2 * j], s[2 * j + 1]), scale2, neg);
+                            if (j % 8 < kPolyOf8) e = exp2_poly(e);
+                            else e = make_float2(ex2(e.x), ex2(e.y));
+                            sum[j & 1] = add2(sum[j & 1], e);
+                            u[j] = pack2<kHalf>(e.x, e.y);
                         }
+                        tmem_st16(tP + col / 2, u);  // where P lies over S: columns that have been read
                     };
-                    if (whole) probabilities(Int<kPolyOf8>());
-                    else probabilities(Int<0>());  // masked scores are -inf and their probabilities exactly 0
+#pragma unroll 1
+                    for (int i = 0; i < 128; i += 64) {
+                        tmem_arrived32(s0);
+                        tmem_ld32(tS + i + 32, s1);
+                        probabilities(s0, i);
+                        tmem_arrived32(s1);
+                        if (i == 0) {
+                            tmem_ld32(tS + 64, s0);
+                        } else if (!C::kAlias) {  // all scores are in registers: the tensor core may write the next ones
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&S.s_free[wg]);
+                        }
+                        probabilities(s1, i + 32);
+                    }
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     tmem_st_wait();
                     tc_fence_before();
-                } else if (!C::kAlias && !(ok = attn_wait(&S.pv_done[wg], pv_par, &S, a.status, 540))) break;
+                } else if (!C::kAlias) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&S.s_free[wg]);
+                    if (!(ok = attn_wait(&S.pv_done[wg], pv_par, &S, a.status, 540))) break;
+                }
                 pv_par ^= 1;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.p_ready[wg]);
