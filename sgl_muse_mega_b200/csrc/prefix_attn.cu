@@ -462,14 +462,19 @@ __device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either i
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
     return r;
 }
+__device__ __forceinline__ float max_nan(float x, float y, float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
 // 2^x for two x on the FMA pipe: x = k + f with k the nearest whole number, 2^f on [-1/2, 1/2] by the polynomial of degree 4 with
-// p(0) = 1 and the least relative error (2.9e-6; a linear program), k added to the exponent. x is kept at or above -127, where
-// the sum of exponents is exactly 0: a masked score (-inf) gives an exact zero. The special-function unit yields 16 results a
-// clock and SM, which would bound the softmax of 64-wide heads; kPolyOf8 of 8 results come from here instead.
+// p(0) = 1 and the least relative error (2.9e-6; a linear program), k added to the exponent. x is kept at or above -126. The
+// special-function unit yields 16 results a clock and SM; kPolyOf8 of 8 results come from here instead, except in tiles with masked
+// keys, whose probabilities have to be exactly 0.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
     const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
-    x.x = fmaxf(x.x, -127.f);
-    x.y = fmaxf(x.y, -127.f);
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
     const float2 r = add2(x, magic);  // k in the low bits
     const float2 f = fma2(add2(r, back), make_float2(-1.f, -1.f), x);
     float2 p = fma2(f, make_float2(0x1.3a007ap-7f, 0x1.3a007ap-7f), make_float2(0x1.c9fd1ep-5f, 0x1.c9fd1ep-5f));
@@ -478,7 +483,11 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
     p = fma2(p, f, make_float2(1.f, 1.f));
     return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
-constexpr int kPolyOf8 = 3;
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+constexpr int kPolyOf8 = 2;
 
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -596,7 +605,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
     if (warp < 8) {
         // ---- softmax ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int wg = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 (warp % 4) lanes in bits 16 ..
         const uint32_t tS = tmem + lanes + C::kS + wg * 128, tP = tmem + lanes + C::kP + wg * C::kPStep, tO = tmem + lanes + C::kO + wg * C::kOStep;
@@ -644,24 +652,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                         if (!whole) hide(s, col);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            mx[0] = max_nan(mx[0], max_nan(s[i], s[i + 1]));
-                            mx[1] = max_nan(mx[1], max_nan(s[i + 2], s[i + 3]));
+                            mx[0] = max_nan(mx[0], s[i], s[i + 1]);
+                            mx[1] = max_nan(mx[1], s[i + 2], s[i + 3]);
                         }
                     };
                     tmem_ld32(tS, s0);
+                    tmem_ld32(tS + 32, s1);
 #pragma unroll 1
                     for (int i = 0; i < 128; i += 64) {
                         tmem_arrived32(s0);
-                        tmem_ld32(tS + i + 32, s1);
-                        highest(s0, i);
                         tmem_arrived32(s1);
-                        tmem_ld32(tS + ((i + 64) & 127), s0);  // at the end: the first columns again, for the second pass
+                        highest(s0, i);
                         highest(s1, i + 32);
+                        tmem_ld32(tS + ((i + 64) & 127), s0);  // at the end: the first columns again, for the second pass
+                        tmem_ld32(tS + ((i + 64) & 127) + 32, s1);
                     }
                     const float top = max_nan(mx[0], mx[1]) * a.scale_log2;
                     if (!(top < INFINITY)) l = NAN;  // a score that is NaN or +inf: so is the row's softmax
                     // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
-                    // P's type and the f32 sums carry without loss), so O is seldom rescaled.
+                    // P's type and the f32 sums carry without loss), so O is seldom rescaled. (m = the maximum
+                    // where it moves: a key that carries the row has p = 1, which P's type holds exactly.)
                     const bool grow = top > m + 8.f;
                     const bool any = __any_sync(0xffffffffu, grow);
                     const float mn = grow ? top : m, f = grow ? ex2(m - mn) : 1.f;  // m = -inf: the factor is 0
@@ -683,36 +693,46 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     }
                     const float ms = m == -INFINITY ? 0.f : m;
                     const float2 neg = make_float2(-ms, -ms);
-                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    auto probabilities = [&](float* s, int col) {
-                        if (!whole) hide(s, col);
-                        uint32_t u[16];
+                    float2 sum[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
+                    auto probabilities = [&](float* s, uint32_t* u, auto poly) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             float2 e = fma2(make_float2(s[2 * j], s[2 * j + 1]), scale2, neg);
-                            if (j % 8 < kPolyOf8) e = exp2_poly(e);
+                            if (j % 8 < decltype(poly)::value) e = exp2_poly(e);
                             else e = make_float2(ex2(e.x), ex2(e.y));
-                            sum[j & 1] = add2(sum[j & 1], e);
+                            sum[j & 3] = add2(sum[j & 3], e);
                             u[j] = pack2<kHalf>(e.x, e.y);
                         }
-                        tmem_st16(tP + col / 2, u);  // where P lies over S: columns that have been read
                     };
 #pragma unroll 1
                     for (int i = 0; i < 128; i += 64) {
                         tmem_arrived32(s0);
-                        tmem_ld32(tS + i + 32, s1);
-                        probabilities(s0, i);
                         tmem_arrived32(s1);
-                        if (i == 0) {
-                            tmem_ld32(tS + 64, s0);
-                        } else if (!C::kAlias) {  // all scores are in registers: the tensor core may write the next ones
+                        if (i != 0 && !C::kAlias) {  // all scores are in registers: the tensor core may write the next ones
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&S.s_free[wg]);
                         }
-                        probabilities(s1, i + 32);
+                        uint32_t u0[16], u1[16];
+                        if (whole) {
+                            probabilities(s0, u0, Int<kPolyOf8>());
+                            probabilities(s1, u1, Int<kPolyOf8>());
+                        } else {
+                            hide(s0, i);
+                            hide(s1, i + 32);
+                            probabilities(s0, u0, Int<0>());
+                            probabilities(s1, u1, Int<0>());
+                        }
+                        if (i == 0) {
+                            tmem_ld32(tS + 64, s0);
+                            tmem_ld32(tS + 96, s1);
+                        }
+                        tmem_st16(tP + i / 2, u0);  // where P lies over S: columns that have been read
+                        tmem_st16(tP + i / 2 + 16, u1);
                     }
-                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
                     tmem_st_wait();
                     tc_fence_before();
                 } else if (!C::kAlias) {
@@ -756,7 +776,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
     } else if (warp == 8) {
         // ---- S = Q K^T ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         constexpr uint32_t id_s = idesc_f16(kHalf, false, kTile);
         // What the issuing thread hands to the tensor core is made uniform over the warp first (shuffles from lane 0): the
         // compiler then keeps descriptors in uniform registers.
@@ -802,7 +821,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     } else if (warp == 11) {
         // ---- O += P V: a warp of its own, because one thread that issued both products and kept both sides' barriers spent
         // more time on those than the products take ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         constexpr uint32_t id_o = idesc_f16(kHalf, true, D);
         const uint64_t v_desc = desc_v(smem_u32(Vs));
         unsigned n = 0, vi = 0, vpar = 0;
@@ -839,7 +857,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         // Where pages hold runs of 8 or more aligned rows, a lane copies a run as one box; else a lane gathers four rows. Rows
         // past the piece's last key are asked for behind the pool's end, which reads zeros: a probability of zero times
         // whatever a stale row holds would not be zero. So the run that the last key ends in is gathered row by row (V).
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const bool is_v = warp == 10;
         const CUtensorMap *run_map = is_v ? &maps.v_run : &maps.k_run, *row_map = is_v ? &maps.v_row : &maps.k_row;
         unsigned char* ring = is_v ? Vs : Ks;
