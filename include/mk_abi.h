@@ -815,7 +815,7 @@ typedef struct MkPrefixAttnBind {
     int64_t window;
     double scale;
     int64_t fp16;
-    uint64_t ws;           // ws_bytes of scratch (mk_prefix_attn_constants), 256-byte aligned
+    uint64_t ws;           // ws_bytes of scratch (mk_prefix_attn_constants), 16-byte aligned
     int64_t ws_bytes;
     uint64_t status;
 } MkPrefixAttnBind;

@@ -70,19 +70,22 @@ __device__ __forceinline__ unsigned own_tiles(const PrefixAttnArgs& a, const Req
     return (unsigned)(r.len - own_start(a, r, prefix) + kTile - 1) / kTile;
 }
 __device__ __forceinline__ int row_blocks(int rows) { return (rows + 2 * kTile - 1) / (2 * kTile); }
+// steps that an item costs besides its tiles
+__device__ __forceinline__ unsigned lead(const PrefixAttnArgs& a, bool pair) { return kItemSteps + (pair ? a.pair_steps : 0); }
 // steps of all row blocks of `rows` rows over `tiles` key tiles, for one kv head
-__device__ __forceinline__ unsigned head_steps(unsigned tiles, int rows) {
-    return tiles > 0 ? tiles * steps_of_rows(rows) + row_blocks(rows) * kItemSteps : 0u;
+__device__ __forceinline__ unsigned head_steps(const PrefixAttnArgs& a, unsigned tiles, int rows) {
+    const unsigned pairs = (rows + kTile - 1) / (2 * kTile);  // blocks of more than kTile rows
+    return tiles > 0 ? tiles * steps_of_rows(rows) + row_blocks(rows) * kItemSteps + pairs * a.pair_steps : 0u;
 }
 __device__ __forceinline__ unsigned own_steps(const PrefixAttnArgs& a, const Req& r, int prefix) {
-    return head_steps(own_tiles(a, r, prefix), r.n * a.G) * a.kvh;
+    return head_steps(a, own_tiles(a, r, prefix), r.n * a.G) * a.kvh;
 }
 __device__ __forceinline__ int own_items(const PrefixAttnArgs& a, const Req& r) { return row_blocks(r.n * a.G) * a.kvh; }
 // the key tiles of an item that the steps [lo, hi) of it stand for; a range that ends inside a pair of steps leaves the pair
 // to the range that starts it
-__device__ __forceinline__ void tiles_of(unsigned lo, unsigned hi, int sh, unsigned& t0, unsigned& t1) {
-    t0 = ((lo > kItemSteps ? lo - kItemSteps : 0u) + sh) >> sh;
-    t1 = ((hi > kItemSteps ? hi - kItemSteps : 0u) + sh) >> sh;
+__device__ __forceinline__ void tiles_of(unsigned lo, unsigned hi, unsigned lead, int sh, unsigned& t0, unsigned& t1) {
+    t0 = ((lo > lead ? lo - lead : 0u) + sh) >> sh;
+    t1 = ((hi > lead ? hi - lead : 0u) + sh) >> sh;
 }
 
 struct Plan {
@@ -183,7 +186,7 @@ __device__ __forceinline__ Plan make_plan(const PrefixAttnArgs& a, const Lens& l
     p.ref = p.prefix > 0 ? ref : 0;
     p.p_lo = p.prefix > 0 ? lo / kTile * kTile : 0;
     p.tiles = p.prefix > 0 && hi > p.p_lo ? (unsigned)(hi - p.p_lo + kTile - 1) / kTile : 0u;
-    p.per_head = head_steps(p.tiles, p.tokens * a.G);
+    p.per_head = head_steps(a, p.tiles, p.tokens * a.G);
     p.prefix_steps = p.per_head * a.kvh;
     unsigned sum = 0;
     if (cum == nullptr) {
@@ -286,7 +289,7 @@ struct Walker {
             });
         }
         load();
-        const unsigned per_head = head_steps(tiles, row_total), block = 2 * tiles + kItemSteps;
+        const unsigned per_head = head_steps(a, tiles, row_total), block = 2 * tiles + lead(a, true);
         h = (int)(pos / per_head);
         pos -= h * per_head;
         rb = (int)(pos / block);
@@ -324,8 +327,8 @@ struct Walker {
             x.key0 = key0;
             x.index = (b < 0 ? 0 : items) + h * blocks + rb;
             const int sh = x.rows > kTile ? 1 : 0;
-            const unsigned len = (tiles << sh) + kItemSteps, stop = min(off + left, len);
-            tiles_of(off, stop, sh, x.t0, x.t1);
+            const unsigned front = lead(a, sh != 0), len = (tiles << sh) + front, stop = min(off + left, len);
+            tiles_of(off, stop, front, sh, x.t0, x.t1);
             left -= stop - off;
             off = 0;
             if (++rb == blocks) rb = 0, ++h;
@@ -992,7 +995,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
 
     // the prefix item and the own item: first step, steps, first CTA and number of candidates, slot of CTA 0, place of the row
     struct Item {
-        unsigned first, len;
+        unsigned first, len, front;
         int sh, c0, n, index, R, row, half;
     };
     const bool alone = h.total < kCtas;  // one step a CTA: no second parts
@@ -1000,13 +1003,14 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
         Item e;
         const int block = gr / (2 * kTile), rr = gr - block * 2 * kTile, left = min(2 * kTile, rows - block * 2 * kTile);
         e.sh = left > kTile ? 1 : 0;
-        e.first = first + kv * head_steps(tiles, rows) + block * (2 * tiles + kItemSteps);
-        e.len = (tiles << e.sh) + kItemSteps;
+        e.front = lead(a, e.sh != 0);
+        e.first = first + kv * head_steps(a, tiles, rows) + block * (2 * tiles + lead(a, true));
+        e.len = (tiles << e.sh) + e.front;
         e.index = index + kv * row_blocks(rows) + block;
         e.R = R;
         e.row = rr & (kTile - 1);
         e.half = rr >> 7;
-        e.c0 = tiles > 0 ? cta_of(e.first + kItemSteps, h.total) : 0;
+        e.c0 = tiles > 0 ? cta_of(e.first + e.front, h.total) : 0;
         e.n = tiles > 0 ? (cta_of(e.first + e.len - 1, h.total) - e.c0 + 1) << (e.sh || alone ? 0 : 1) : 0;
         return e;
     };
@@ -1024,7 +1028,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
         if (q < n) {
             const unsigned lo = max(range_lo(h.total, c), first), hi = min(range_lo(h.total, c + 1), first + len);
             unsigned t0 = 0, t1 = 0;
-            if (hi > lo) tiles_of(lo - first, hi - first, sh, t0, t1);
+            if (hi > lo) tiles_of(lo - first, hi - first, own ? ind.front : pre.front, sh, t0, t1);
             on = t1 > t0 + (sh != 0 ? 0 : s);
         }
         const float4* src =

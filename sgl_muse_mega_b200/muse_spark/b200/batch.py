@@ -80,6 +80,8 @@ class BlockTables:
         _check("pages_owned", pages_owned, i32, (pool,), dev)
         _check("free_pages", free_pages, i32, (None,), dev)
         _check("free_words", free_words, i64, (2,), dev)
+        if batch < 1 or rows < 1:
+            raise ValueError(f"batch {batch} / rows {rows}: at least one of each")
         self.block_table = torch.full((batch, width), -1, dtype=i32, device=dev)
         self.slots = _z(rows, dtype=i64, device=dev)
         self.positions = _z(rows, dtype=i64, device=dev)
