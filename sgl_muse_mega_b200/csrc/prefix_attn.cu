@@ -490,7 +490,7 @@ template <int N>
 struct Int {
     static constexpr int value = N;
 };
-constexpr int kPolyOf8 = 2;
+constexpr int kPolyOf8 = 1;
 
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -975,11 +975,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 // ---- merge --------------------------------------------------------------------------------------------------------------
 // out = sum O_i 2^(m_i - M) / L over the pieces of the row's prefix item and own item, M = max m_i, L = sum l_i 2^(m_i - M). A
 // warp takes one row. Its lanes look up a candidate piece each (a CTA of the item's range, a part of its slot): which slot, m
-// and l, all requested at once; then D / 4 lanes read a piece's O (a float4 each), eight loads in flight, in the order of the
+// and l, all requested at once; then D / 4 lanes read a piece's O (a float4 each), four loads in flight, in the order of the
 // candidates. What rests on the lengths alone is done before the wait for the first kernel. The time is the chain of
 // three round trips to L2 (plan, m and l, O) behind that kernel's end.
 template <int D, bool kHalf>
-__global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant__ PrefixAttnArgs a) {
+__global__ void __launch_bounds__(256, 3) prefix_merge_kernel(const __grid_constant__ PrefixAttnArgs a) {
     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;  // lanes of a piece, pieces read side by side
     const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
@@ -1044,7 +1044,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const __grid_constant
         bool weighed = false;
         float g = 0.f;
         while (there != 0u) {  // O is asked for before m and l are looked at
-            constexpr int kAhead = 8;
+            constexpr int kAhead = 4;
             float4 v[kAhead];
             int from[kAhead];
 #pragma unroll
