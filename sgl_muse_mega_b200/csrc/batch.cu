@@ -269,10 +269,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     typedef Pair<T> P2;
     typedef typename P2::type T2;
     griddep_wait();
-    // Nothing waits for anything it does not need: the row's words and the first heads are asked for together, the table row
-    // follows the position, the checks come behind all loads (the row lies inside the tensors whether it is live or not).
+    // Rows that are not live cost one word. Nothing else waits for what it does not need: the row's words and the first heads
+    // are asked for together, the table row follows the position, the checks come behind all loads.
     const int r = blockIdx.x;
-    const int n_rows = a.n_rows != nullptr ? *a.n_rows : a.rows;
+    if (a.n_rows != nullptr && r >= *a.n_rows) return;
     long long pos = a.positions[r];
     long long slot = a.k_cache != nullptr ? a.slots[r] : -1;
     const T* qr = (const T*)a.q + r * a.q_row;
@@ -305,7 +305,6 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     const int vp = a.dim / 8, v0 = blockDim.x - 1 - threadIdx.x;
     uint4 vw = make_uint4(0, 0, 0, 0);
     if (a.v != nullptr && v0 < a.kvh * vp) vw = *(const uint4*)(vr + v0 / vp * a.v_head + v0 % vp * 8);
-    if (r >= n_rows) return;
     if (pos < 0 || pos >= a.cos_rows) {
         if (threadIdx.x == 0) batch_status(a.status, 4, 510, (int)pos, (int)min(a.cos_rows, 0x7fffffffll));
         pos = 0;

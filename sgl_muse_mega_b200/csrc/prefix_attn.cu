@@ -348,16 +348,16 @@ template <int D>
 struct Cfg {
     static constexpr int kAtoms = D / 64;                 // 64-wide column blocks of a K / V tile
     static constexpr int kTileBytes = kTile * D * 2;      // K, V or Q tile
-    static constexpr int kRing = D == 64 ? 4 : 2;         // K stages and V stages
+    static constexpr int kRingK = D == 64 ? 4 : 2, kRingV = D == 64 ? 4 : 2;  // K stages, V stages
     static constexpr int kQ = D == 64 ? 4 : 3;            // query tiles
-    static constexpr int kSmem = (2 * kRing + kQ) * kTileBytes + 1024;
+    static constexpr int kSmem = (kRingK + kRingV + kQ) * kTileBytes + 1024;
     static constexpr bool kAlias = D == 128;              // P over S: tensor memory holds 2 x (128 + 128) columns then
     // tensor-memory columns (512): S of each warpgroup, P, O
     static constexpr uint32_t kS = 0, kP = D == 64 ? 256 : 0, kPStep = D == 64 ? 64 : 128, kO = D == 64 ? 384 : 256, kOStep = D;
 };
 
 struct Bars {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[4], q_empty[4];
+    uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6], q_full[6], q_empty[6];
     uint64_t s_full[2], s_free[2], p_ready[2], o_full[2], pv_done[2];
     uint64_t drain[2];
     uint32_t tmem;
@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     __shared__ Bars S;
     unsigned char* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     unsigned char* Ks = smem;
-    unsigned char* Vs = Ks + C::kRing * C::kTileBytes;
-    unsigned char* Qs = Vs + C::kRing * C::kTileBytes;
+    unsigned char* Vs = Ks + C::kRingK * C::kTileBytes;
+    unsigned char* Qs = Vs + C::kRingV * C::kTileBytes;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_wait();
     Lens lens;
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (lane < 4 || a.q_box) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
     if (tid == 0) {
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 6; ++i) {
             mbar_init(&S.k_full[i], 1);
             mbar_init(&S.k_empty[i], 1);
             mbar_init(&S.v_full[i], 1);
@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     if (st + tiles_q >= ns) tc_commit(&S.q_empty[qs]);
                 }
                 __syncwarp();
-                if (last_k && ++ki == C::kRing) ki = 0, kpar ^= 1;
+                if (last_k && ++ki == C::kRingK) ki = 0, kpar ^= 1;
             }
             qi += tiles_q;
             if (qi >= C::kQ) qi -= C::kQ, qpar ^= 1;
@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     if (st + 2 >= ns) tc_commit(&S.o_full[w]);
                 }
                 __syncwarp();
-                if (last_v && ++vi == C::kRing) vi = 0, vpar ^= 1;
+                if (last_v && ++vi == C::kRingV) vi = 0, vpar ^= 1;
             }
         }
         if (elect_one()) tc_commit(&S.drain[1]);
@@ -864,6 +864,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const CUtensorMap *run_map = is_v ? &maps.v_run : &maps.k_run, *row_map = is_v ? &maps.v_row : &maps.k_row;
         unsigned char* ring = is_v ? Vs : Ks;
         uint64_t *full = is_v ? S.v_full : S.k_full, *empty = is_v ? S.v_empty : S.k_empty;
+        const unsigned stages = is_v ? C::kRingV : C::kRingK;
+        unsigned place = 0, phase = 0;  // of the ring
         const int head = is_v ? a.v_head : a.k_head;
         const bool runs = a.run >= 8;
         const int per = runs ? a.run : 4, mine = lane * per;  // this lane's keys of a tile
@@ -922,8 +924,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
             if (!ok) break;
             for (unsigned t = x.t0; t < x.t1; ++t) {
-                const unsigned i = issued % C::kRing;
-                if (!(ok = attn_wait(&empty[i], ((issued / C::kRing) & 1) ^ 1, &S, a.status, 537))) break;
+                const unsigned i = place;
+                if (!(ok = attn_wait(&empty[i], phase ^ 1, &S, a.status, 537))) break;
                 if (lane == 0) mbar_arrive_expect_tx(&full[i], C::kTileBytes);
                 __syncwarp();
                 unsigned char* dst = ring + i * C::kTileBytes + mine * 128;
@@ -948,6 +950,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     }
                 }
                 ++issued;
+                if (++place == stages) place = 0, phase ^= 1;
                 if (t + 1 < x.t1) slots_of(t + 1, y);
             }
         }
@@ -967,7 +970,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 }
             }
         };
-        landed(warp == 10 ? S.v_full : S.k_full, C::kRing, issued);
+        landed(warp == 10 ? S.v_full : S.k_full, warp == 10 ? C::kRingV : C::kRingK, issued);
         if (warp == 9) landed(S.q_full, C::kQ, q_count);
     }
 }
@@ -981,116 +984,121 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 template <int D, bool kHalf>
 __global__ void __launch_bounds__(256, 3) prefix_merge_kernel(const __grid_constant__ PrefixAttnArgs a) {
     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;  // lanes of a piece, pieces read side by side
-    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
-    const bool inside = tok < a.rows;
-    const int b = request_of_warp(a, inside ? tok : 0, lane);
-    const Req r = request(a, b);
-    const int j = tok - r.first, kv = head / a.G, hg = head - kv * a.G;
-    griddep_wait();
-    const unsigned* cum = (const unsigned*)(a.ws + 256);
-    const PlanHead h = *(const PlanHead*)a.ws;
-    const unsigned cum_step = cum[b], cum_item = cum[a.batch + b];
-    if (!inside || tok >= (int)h.tokens || j < 0 || j >= r.n) return;
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)a.rows * a.qh;
+    bool waited = false;
+    for (long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); id < rows; id += (long long)gridDim.x * 8) {
+        const int tok = (int)(id / a.qh), head = (int)(id - (long long)tok * a.qh);
+        const int b = request_of_warp(a, tok, lane);
+        const Req r = request(a, b);
+        const int j = tok - r.first, kv = head / a.G, hg = head - kv * a.G;
+        if (!waited) griddep_wait();
+        waited = true;
+        const unsigned* cum = (const unsigned*)(a.ws + 256);
+        const PlanHead h = *(const PlanHead*)a.ws;
+        const unsigned cum_step = cum[b], cum_item = cum[a.batch + b];
+        if (tok >= (int)h.tokens) return;  // so are all later ones
+        if (j < 0 || j >= r.n) continue;
 
-    // the prefix item and the own item: first step, steps, first CTA and number of candidates, slot of CTA 0, place of the row
-    struct Item {
-        unsigned first, len, front;
-        int sh, c0, n, index, R, row, half;
-    };
-    const bool alone = h.total < kCtas;  // one step a CTA: no second parts
-    auto item = [&](unsigned tiles, int rows, int gr, unsigned first, int index, int R) {
-        Item e;
-        const int block = gr / (2 * kTile), rr = gr - block * 2 * kTile, left = min(2 * kTile, rows - block * 2 * kTile);
-        e.sh = left > kTile ? 1 : 0;
-        e.front = lead(a, e.sh != 0);
-        e.first = first + kv * head_steps(a, tiles, rows) + block * (2 * tiles + lead(a, true));
-        e.len = (tiles << e.sh) + e.front;
-        e.index = index + kv * row_blocks(rows) + block;
-        e.R = R;
-        e.row = rr & (kTile - 1);
-        e.half = rr >> 7;
-        e.c0 = tiles > 0 ? cta_of(e.first + e.front, h.total) : 0;
-        e.n = tiles > 0 ? (cta_of(e.first + e.len - 1, h.total) - e.c0 + 1) << (e.sh || alone ? 0 : 1) : 0;
-        return e;
-    };
-    const Item pre = item(h.tiles, (int)h.tokens * a.G, tok * a.G + hg, 0u, 0, kTile);
-    const Item ind = item(own_tiles(a, r, (int)h.prefix), r.n * a.G, j * a.G + hg, cum_step, (int)cum_item, a.suffix_rows);
-    float M = -INFINITY, Ls = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < pre.n + ind.n; k0 += 32) {
-        const int k = k0 + lane;
-        const bool own = k >= pre.n;
-        const int q = own ? k - pre.n : k, n = own ? ind.n : pre.n, sh = own ? ind.sh : pre.sh, R = own ? ind.R : pre.R, row = own ? ind.row : pre.row;
-        const bool one = sh != 0 || alone;
-        const int c = (own ? ind.c0 : pre.c0) + (one ? q : q >> 1), s = sh != 0 ? (own ? ind.half : pre.half) : one ? 0 : q & 1;
-        const unsigned first = own ? ind.first : pre.first, len = own ? ind.len : pre.len;
-        bool on = false;
-        if (q < n) {
-            const unsigned lo = max(range_lo(h.total, c), first), hi = min(range_lo(h.total, c + 1), first + len);
-            unsigned t0 = 0, t1 = 0;
-            if (hi > lo) tiles_of(lo - first, hi - first, own ? ind.front : pre.front, sh, t0, t1);
-            on = t1 > t0 + (sh != 0 ? 0 : s);
-        }
-        const float4* src =
-            (const float4*)(a.ws + (own ? a.ws_suffix : a.ws_prefix) + ((long long)((own ? ind.index : pre.index) + c) * 2 + s) * part_bytes(R, D)) + row;
-        float m = -INFINITY, l = 0.f;
-        if (on) {
-            const float* ml = (const float*)(src - row + R * (D / 4)) + row;
-            m = ml[0];
-            l = ml[R];
-        }
-        unsigned there = __ballot_sync(0xffffffffu, on);
-        const unsigned owned = __ballot_sync(0xffffffffu, own);
-        bool weighed = false;
-        float g = 0.f;
-        while (there != 0u) {  // O is asked for before m and l are looked at
-            constexpr int kAhead = 4;
-            float4 v[kAhead];
-            int from[kAhead];
+        // the prefix item and the own item: first step, steps, first CTA and number of candidates, slot of CTA 0, place of the row
+        struct Item {
+            unsigned first, len, front;
+            int sh, c0, n, index, R, row, half;
+        };
+        const bool alone = h.total < kCtas;  // one step a CTA: no second parts
+        auto item = [&](unsigned tiles, int rows, int gr, unsigned first, int index, int R) {
+            Item e;
+            const int block = gr / (2 * kTile), rr = gr - block * 2 * kTile, left = min(2 * kTile, rows - block * 2 * kTile);
+            e.sh = left > kTile ? 1 : 0;
+            e.front = lead(a, e.sh != 0);
+            e.first = first + kv * head_steps(a, tiles, rows) + block * (2 * tiles + lead(a, true));
+            e.len = (tiles << e.sh) + e.front;
+            e.index = index + kv * row_blocks(rows) + block;
+            e.R = R;
+            e.row = rr & (kTile - 1);
+            e.half = rr >> 7;
+            e.c0 = tiles > 0 ? cta_of(e.first + e.front, h.total) : 0;
+            e.n = tiles > 0 ? (cta_of(e.first + e.len - 1, h.total) - e.c0 + 1) << (e.sh || alone ? 0 : 1) : 0;
+            return e;
+        };
+        const Item pre = item(h.tiles, (int)h.tokens * a.G, tok * a.G + hg, 0u, 0, kTile);
+        const Item ind = item(own_tiles(a, r, (int)h.prefix), r.n * a.G, j * a.G + hg, cum_step, (int)cum_item, a.suffix_rows);
+        float M = -INFINITY, Ls = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < pre.n + ind.n; k0 += 32) {
+            const int k = k0 + lane;
+            const bool own = k >= pre.n;
+            const int q = own ? k - pre.n : k, n = own ? ind.n : pre.n, sh = own ? ind.sh : pre.sh, R = own ? ind.R : pre.R, row = own ? ind.row : pre.row;
+            const bool one = sh != 0 || alone;
+            const int c = (own ? ind.c0 : pre.c0) + (one ? q : q >> 1), s = sh != 0 ? (own ? ind.half : pre.half) : one ? 0 : q & 1;
+            const unsigned first = own ? ind.first : pre.first, len = own ? ind.len : pre.len;
+            bool on = false;
+            if (q < n) {
+                const unsigned lo = max(range_lo(h.total, c), first), hi = min(range_lo(h.total, c + 1), first + len);
+                unsigned t0 = 0, t1 = 0;
+                if (hi > lo) tiles_of(lo - first, hi - first, own ? ind.front : pre.front, sh, t0, t1);
+                on = t1 > t0 + (sh != 0 ? 0 : s);
+            }
+            const float4* src =
+                (const float4*)(a.ws + (own ? a.ws_suffix : a.ws_prefix) + ((long long)((own ? ind.index : pre.index) + c) * 2 + s) * part_bytes(R, D)) + row;
+            float m = -INFINITY, l = 0.f;
+            if (on) {
+                const float* ml = (const float*)(src - row + R * (D / 4)) + row;
+                m = ml[0];
+                l = ml[R];
+            }
+            unsigned there = __ballot_sync(0xffffffffu, on);
+            const unsigned owned = __ballot_sync(0xffffffffu, own);
+            bool weighed = false;
+            float g = 0.f;
+            while (there != 0u) {  // O is asked for before m and l are looked at
+                constexpr int kAhead = 4;
+                float4 v[kAhead];
+                int from[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                from[i] = 32;
+                for (int i = 0; i < kAhead; ++i) {
+                    from[i] = 32;
 #pragma unroll
-                for (int y = 0; y < kAtOnce; ++y) {
-                    const int f = there != 0u ? __ffs(there) - 1 : 32;
-                    there &= there - 1;
-                    if (lane / kLanes == y) from[i] = f;
+                    for (int y = 0; y < kAtOnce; ++y) {
+                        const int f = there != 0u ? __ffs(there) - 1 : 32;
+                        there &= there - 1;
+                        if (lane / kLanes == y) from[i] = f;
+                    }
+                    const float4* p = (const float4*)__shfl_sync(0xffffffffu, (unsigned long long)src, from[i] & 31);
+                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (from[i] < 32) v[i] = p[(lane % kLanes) * ((owned >> from[i]) & 1u ? a.suffix_rows : kTile)];
                 }
-                const float4* p = (const float4*)__shfl_sync(0xffffffffu, (unsigned long long)src, from[i] & 31);
-                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (from[i] < 32) v[i] = p[(lane % kLanes) * ((owned >> from[i]) & 1u ? a.suffix_rows : kTile)];
-            }
-            if (!weighed) {
-                weighed = true;
-                const float mn = fmaxf(M, warp_max(m));
-                const float f = M == mn ? 1.f : ex2(M - mn);   // of what is there
-                g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
-                M = mn;
-                Ls = Ls * f + warp_sum(l * g);
+                if (!weighed) {
+                    weighed = true;
+                    const float mn = fmaxf(M, warp_max(m));
+                    const float f = M == mn ? 1.f : ex2(M - mn);   // of what is there
+                    g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
+                    M = mn;
+                    Ls = Ls * f + warp_sum(l * g);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] *= f;
-            }
+                    for (int i = 0; i < 4; ++i) o[i] *= f;
+                }
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const float w = __shfl_sync(0xffffffffu, g, from[i] & 31);
-                if (from[i] < 32 && w != 0.f) {
-                    o[0] += v[i].x * w;
-                    o[1] += v[i].y * w;
-                    o[2] += v[i].z * w;
-                    o[3] += v[i].w * w;
+                for (int i = 0; i < kAhead; ++i) {
+                    const float w = __shfl_sync(0xffffffffu, g, from[i] & 31);
+                    if (from[i] < 32 && w != 0.f) {
+                        o[0] += v[i].x * w;
+                        o[1] += v[i].y * w;
+                        o[2] += v[i].z * w;
+                        o[3] += v[i].w * w;
+                    }
                 }
             }
         }
-    }
-    if (kAtOnce == 2) {
+        if (kAtOnce == 2) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 16);
+            for (int i = 0; i < 4; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 16);
+        }
+        const float inv = Ls == 0.f ? 0.f : 1.f / Ls;  // a row that saw no key is zero
+        if (lane < kLanes)
+            *(uint2*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * 4) * 2) =
+                make_uint2(pack2<kHalf>(o[0] * inv, o[1] * inv), pack2<kHalf>(o[2] * inv, o[3] * inv));
+        if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + log2f(Ls)) * kLn2;
     }
-    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;  // a row that saw no key is zero
-    if (lane < kLanes)
-        *(uint2*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * 4) * 2) =
-            make_uint2(pack2<kHalf>(o[0] * inv, o[1] * inv), pack2<kHalf>(o[2] * inv, o[3] * inv));
-    if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + log2f(Ls)) * kLn2;
 }
 
 template <int D, bool kHalf>
@@ -1107,7 +1115,9 @@ static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const PrefixAttnMaps
     cfg.numAttrs = pdl ? 1 : 0;
     cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_attn_kernel<D, kHalf>, a, maps);
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3((unsigned)(((long long)a.rows * a.qh + 7) / 8));
+    // at most four rounds of three blocks an SM: rows beyond the batch's must not cost a block each
+    const long long blocks = ((long long)a.rows * a.qh + 7) / 8, most = 12ll * kCtas;
+    cfg.gridDim = dim3((unsigned)(blocks < most ? blocks : most));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;  // its wait is its first statement, so it may always start under the first kernel's tail
