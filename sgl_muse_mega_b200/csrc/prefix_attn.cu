@@ -406,11 +406,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uin
         : "r"(d), "r"(at), "l"(bd), "r"(idesc), "r"(acc)
         : "memory");
 }
-// f32 accumulator, A and B f16 (0) or bf16 (1), A K-major, B K-major or (bit 16) N-major, M = 128
-__host__ __device__ constexpr uint32_t idesc_f16(bool half, bool b_n_major, int n) {
+// f32 accumulator, A and B f16 (0) or bf16 (1), A K-major, B K-major or (bit 16) N-major
+__host__ __device__ constexpr uint32_t idesc_f16(bool half, bool b_n_major, int m, int n) {
     return (1u << 4) | ((half ? 0u : 1u) << 7) | ((half ? 0u : 1u) << 10) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
-           ((128u >> 4) << 24);
+           ((uint32_t)(m >> 4) << 24);
 }
+// An item of at most 16 rows takes products of 64 rows instead of 128: rows 0 .. 15 lie in the same lanes in both shapes, and the
+// tensor core does half the padding's work. (96 decodes over their own 2 K keys, which run at the board's power limit: 187 -> 175 us
+// in a long run, 161 -> 157 us in a short one.)
+constexpr int kFew = 16;
 // V as the N-major operand: 64 columns (128 bytes, swizzled) x 8 keys form an atom of 1024 bytes; the next 8 keys follow
 // it (stride offset), the next 64 columns lie a whole tile of 128-byte rows further (leading offset)
 __device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
@@ -675,7 +679,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
                     // P's type and the f32 sums carry without loss), so O is seldom rescaled. (m = the maximum
                     // where it moves: a key that carries the row has p = 1, which P's type holds exactly.)
-                    const bool grow = top > m + 8.f;
+                    const bool grow = top > m + 8.f && rr < x.rows;
                     const bool any = __any_sync(0xffffffffu, grow);
                     const float mn = grow ? top : m, f = grow ? ex2(m - mn) : 1.f;  // m = -inf: the factor is 0
                     m = mn;
@@ -779,7 +783,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
     } else if (warp == 8) {
         // ---- S = Q K^T ----
-        constexpr uint32_t id_s = idesc_f16(kHalf, false, kTile);
         // What the issuing thread hands to the tensor core is made uniform over the warp first (shuffles from lane 0): the
         // compiler then keeps descriptors in uniform registers.
         const uint64_t q_desc = desc_sw128(smem_u32(Qs)), k_desc = desc_sw128(smem_u32(Ks));
@@ -787,6 +790,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         bool ok = true;
         while (ok && walk.next(x)) {
             const bool pair = x.pair();
+            const uint32_t id_s = __shfl_sync(0xffffffffu, x.rows <= kFew ? idesc_f16(kHalf, false, 64, kTile) : idesc_f16(kHalf, false, kTile, kTile), 0);
             const unsigned ns = x.steps(), tiles_q = pair ? 2 : 1;
             for (unsigned st = 0; st < ns; ++st, ++n) {
                 const int w = __shfl_sync(0xffffffffu, (int)(n & 1), 0);
@@ -824,12 +828,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     } else if (warp == 11) {
         // ---- O += P V: a warp of its own, because one thread that issued both products and kept both sides' barriers spent
         // more time on those than the products take ----
-        constexpr uint32_t id_o = idesc_f16(kHalf, true, D);
         const uint64_t v_desc = desc_v(smem_u32(Vs));
         unsigned n = 0, vi = 0, vpar = 0;
         bool ok = true;
         while (ok && walk.next(x)) {
             const bool pair = x.pair();
+            const uint32_t id_o = __shfl_sync(0xffffffffu, x.rows <= kFew ? idesc_f16(kHalf, true, 64, D) : idesc_f16(kHalf, true, kTile, D), 0);
             const unsigned ns = x.steps();
             for (unsigned st = 0; st < ns; ++st, ++n) {
                 const int w = __shfl_sync(0xffffffffu, (int)(n & 1), 0), vs = __shfl_sync(0xffffffffu, (int)vi, 0);
