@@ -15,10 +15,10 @@
 // item i that CTA c computes goes to slot i + c of the scratch: walking the sequence, every new piece moves to the next
 // item or the next CTA, so the slots are distinct. prefix_merge_kernel adds the pieces of each row, in slot order.
 //
-// A CTA's twelve warps: two softmax warpgroups (a thread holds one query row, its scores are one TMEM lane), one thread
-// that issues the tensor-core products, a warp each that brings in K rows, V rows (TMA boxes of a page's rows, or gathers of
-// four rows where pages are small or odd) and queries. Steps alternate between the two warpgroups, each with its own
-// S, P and O in tensor memory: while one takes the exponentials of its step the tensor core works for the other.
+// A CTA's twelve warps: two softmax warpgroups (a thread holds one query row, its scores are one TMEM lane), a warp that issues
+// the products S = Q K^T, one that issues O += P V, one that brings in queries and K rows, one V rows (TMA boxes of a page's
+// rows, or gathers of four rows where pages are small or odd). Steps alternate between the two warpgroups, each with its
+// own S, P and O in tensor memory: while one takes the exponentials of its step the tensor core works for the other.
 //
 // Measured (whole launch, both kernels): 32 requests x 16 rows over 32 K shared tokens, 16 heads of 64 on 2 kv heads: 120 us = 579 TFLOP/s,
 // bound by the softmax's phases that depend on one another (two steps a CTA take about 3000 cycles, their exponentials 2 x 900 of
@@ -50,7 +50,7 @@ struct Req {
 // the lengths of request b as far as they are usable: what contradicts the launch's extents is left out (and recorded)
 __device__ __forceinline__ Req usable(const PrefixAttnArgs& a, int b, int c0, int c1, int len, int* status) {
     Req r{c0, c1 - c0, len};
-    if (r.n < 0 || r.n > a.max_new || r.first < 0 || r.first + r.n > a.rows) {
+    if (r.n < 0 || r.n > a.max_new || r.first < 0 || r.first > a.rows - r.n) {
         if (status != nullptr) batch_status(status, 4, 520, b, r.n);
         r.n = 0;
     }
@@ -319,7 +319,10 @@ struct Walker {
         while (left > 0) {
             while (tiles == 0 || h == a.kvh) {  // on to the next request that has steps
                 if (b >= 0) items += blocks * a.kvh;
-                ++b;
+                if (++b >= a.batch) {  // only where the lengths changed under the kernel
+                    left = 0;
+                    return false;
+                }
                 h = 0;
                 load();
             }

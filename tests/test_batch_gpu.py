@@ -384,7 +384,8 @@ def test_attention_bad_pages_and_lengths_are_recorded():
     out, _, _ = R.attention(c.q, c.k, c.v, c.table, c.kv, c.cu, 16, 0.125, 0)
     for r in (0, 3):  # the other requests are what they are
         assert (op.out[r].double().cpu() - out[r]).abs().max() < 0.05
-    for bad in (dict(kv_lens=[100, 1 << 20, 90]), dict(cu_rows=[0, 1, 4, 5]), dict(prefix_len=[-3]), dict(cu_rows=[0, 1, 0, 1])):
+    for bad in (dict(kv_lens=[100, 1 << 20, 90]), dict(cu_rows=[0, 1, 4, 5]), dict(prefix_len=[-3]), dict(cu_rows=[0, 1, 0, 1]),
+                dict(cu_rows=[2**31 - 1, -(2**31), 3, 4]), dict(cu_rows=[0, 2**31 - 1, -(2**31), 4]), dict(cu_rows=[-5, -4, -2, 4])):
         c = AttnCase(6, **base)
         op = c.bind()
         for k, v in bad.items():
