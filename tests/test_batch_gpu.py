@@ -74,7 +74,7 @@ def check_tables(op, c, rows, filler=0):
 
 
 @pytest.mark.parametrize("batch,page,ctx_hi,new_hi", [(1, 1, 40, 16), (1, 64, 3000, 700), (5, 16, 200, 1), (33, 7, 90, 40), (260, 16, 64, 3),
-                                                       (64, 128, 9000, 500), (1, 1, 5000, 1)])  # fmt: skip
+                                                       (64, 128, 9000, 500), (1, 1, 5000, 1), (4096, 16, 20, 2)])  # fmt: skip
 def test_tables(batch, page, ctx_hi, new_hi):
     c = tables_case(batch + page, batch, page, ctx_hi, new_hi)
     rows = sum(c["new"]) + 5
@@ -316,6 +316,12 @@ ATTN = {
     "window of one key": dict(kv=[77, 300], new=[3, 1], prefix=0, qh=4, kvh=4, dim=64, page=16, window=1),
     "33 requests": dict(kv=[128 + 5 * i for i in range(33)], new=[1 + i % 3 for i in range(33)], prefix=128, qh=4, kvh=1, dim=64, page=16),
     "130 requests": dict(kv=[130 + i for i in range(130)], new=[1] * 130, prefix=128, qh=8, kvh=1, dim=64, page=128),
+    "700 requests": dict(kv=[(37 * i) % 190 for i in range(700)], new=[min(i % 4, (37 * i) % 190) for i in range(700)], prefix=0, qh=8, kvh=2, dim=64,
+                         page=16),
+    "nothing behind the prefix": dict(kv=[256, 256, 256], new=[1, 4, 2], prefix=256, qh=8, kvh=1, dim=64, page=16),
+    "128 heads a group": dict(kv=[200, 300], new=[2, 1], prefix=160, qh=128, kvh=1, dim=128, page=16),
+    "256 heads a group": dict(kv=[200, 300], new=[2, 1], prefix=0, qh=256, kvh=1, dim=64, page=16),
+    "a million keys": dict(kv=[1000003], new=[2], prefix=0, qh=2, kvh=1, dim=64, page=128),
     "many splits of one item": dict(kv=[30000, 29000], new=[1, 1], prefix=28672, qh=8, kvh=1, dim=64, page=64),
     "tall prefix": dict(kv=[2100] * 9, new=[16] * 9, prefix=2048, qh=16, kvh=1, dim=128, page=128),
 }  # fmt: skip
