@@ -86,7 +86,8 @@ struct PrefixAttnArgs {
     const int* prefix_len;
     int batch, rows, max_new, qh, kvh, G, page, page_shift, kv_rows, window, suffix_rows;
     int k_head, v_head;  // elements between the heads of a cache row
-    int pair_steps;      // what an item of more than 128 rows costs besides its steps, beyond what a smaller one does
+    int item_steps;      // what an item costs besides its steps, counted in steps
+    int pair_steps;      // the same of one of more than 128 rows, beyond that
     int run;             // rows of a copy: the largest power of two up to 128 that divides the page
     int q_box;           // the queries of a tile are 128 / G whole tokens: copied as a box
     float scale_log2;

@@ -35,9 +35,6 @@ using namespace umma;
 constexpr int kTile = 128;  // rows of a step and keys of a tile
 constexpr int kAttnThreads = 384;
 constexpr float kLn2 = 0.69314718055994530942f;
-// What an item costs besides its steps (its queries in, its O out, the tensor core's start), counted in steps. Of 2 / 3 / 4 / 5 / 6:
-// 32 x 16 rows over a 32 K prefix 132 / 127 / 127 / 127 / 129 us, 96 decodes over their own keys 162 / 164 / 165 / 169 / 169.
-constexpr unsigned kItemSteps = 3;
 
 // ---- the plan: the same numbers in every warp of both kernels ---------------------------------------------------------
 struct PlanHead {  // in front of the scratch, for the merge kernel
@@ -76,12 +73,12 @@ __device__ __forceinline__ unsigned own_tiles(const PrefixAttnArgs& a, const Req
     return (unsigned)(r.len - own_start(a, r, prefix) + kTile - 1) / kTile;
 }
 __device__ __forceinline__ int row_blocks(int rows) { return (rows + 2 * kTile - 1) / (2 * kTile); }
-// steps that an item costs besides its tiles
-__device__ __forceinline__ unsigned lead(const PrefixAttnArgs& a, bool pair) { return kItemSteps + (pair ? a.pair_steps : 0); }
+// what an item costs besides its tiles (its queries in, its O out, the tensor core's start), counted in steps
+__device__ __forceinline__ unsigned lead(const PrefixAttnArgs& a, bool pair) { return a.item_steps + (pair ? a.pair_steps : 0); }
 // steps of all row blocks of `rows` rows over `tiles` key tiles, for one kv head
 __device__ __forceinline__ unsigned head_steps(const PrefixAttnArgs& a, unsigned tiles, int rows) {
     const unsigned pairs = (rows + kTile - 1) / (2 * kTile);  // blocks of more than kTile rows
-    return tiles > 0 ? tiles * steps_of_rows(rows) + row_blocks(rows) * kItemSteps + pairs * a.pair_steps : 0u;
+    return tiles > 0 ? tiles * steps_of_rows(rows) + row_blocks(rows) * a.item_steps + pairs * a.pair_steps : 0u;
 }
 __device__ __forceinline__ unsigned own_steps(const PrefixAttnArgs& a, const Req& r, int prefix) {
     return head_steps(a, own_tiles(a, r, prefix), r.n * a.G) * a.kvh;
@@ -657,15 +654,27 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     // maximum, then the probabilities. Loops of few instructions: a step's code unrolled over 128 columns
                     // ran at the pace of instruction fetch where it ran once or twice (a launch of few steps: 4 us a step).
                     const bool whole = __all_sync(0xffffffffu, (lo <= kb && hi >= kb + kTile) || rr >= x.rows);
+                    // Otherwise each half of the columns is looked at: one that no row of the warp sees is passed over, one that
+                    // all see whole needs no mask; in the others a bit a column says what the row sees.
+                    unsigned part = 0, none = 0;  // halves in 64 columns: seen in part, not seen
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int c0 = lo - kb - 64 * i, c1 = hi - kb - 64 * i;
+                            const bool idle = rr >= x.rows;
+                            if (__all_sync(0xffffffffu, c1 <= 0 || c0 >= 64 || c0 >= c1 || idle)) none |= 1u << i;
+                            else if (!__all_sync(0xffffffffu, (c0 <= 0 && c1 >= 64) || idle)) part |= 1u << i;
+                        }
+                    }
                     float s0[32], s1[32];
                     auto hide = [&](float* s, int col) {
-                        const int c0 = lo - kb - col, c1 = hi - kb - col;
+                        const int c0 = max(lo - kb - col, 0), c1 = min(hi - kb - col, 32);
+                        const unsigned see = c0 < c1 ? (0xffffffffu >> (32 - (c1 - c0))) << c0 : 0u;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = i >= c0 && i < c1 ? s[i] : -INFINITY;
+                        for (int i = 0; i < 32; ++i) s[i] = see & (1u << i) ? s[i] : -INFINITY;
                     };
                     float mx[2] = {-INFINITY, -INFINITY};
-                    auto highest = [&](float* s, int col) {
-                        if (!whole) hide(s, col);
+                    auto highest = [&](float* s) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             mx[0] = max_nan(mx[0], s[i], s[i + 1]);
@@ -674,15 +683,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     };
                     tmem_ld32(tS, s0);
                     tmem_ld32(tS + 32, s1);
+                    auto first_pass = [&](auto masks) {
 #pragma unroll 1
-                    for (int i = 0; i < 128; i += 64) {
-                        tmem_arrived32(s0);
-                        tmem_arrived32(s1);
-                        highest(s0, i);
-                        highest(s1, i + 32);
-                        tmem_ld32(tS + ((i + 64) & 127), s0);  // at the end: the first columns again, for the second pass
-                        tmem_ld32(tS + ((i + 64) & 127) + 32, s1);
-                    }
+                        for (int i = 0; i < 128; i += 64) {
+                            tmem_arrived32(s0);
+                            tmem_arrived32(s1);
+                            if (decltype(masks)::value && ((part | none) & (i == 0 ? 1u : 2u))) {
+                                hide(s0, i);
+                                hide(s1, i + 32);
+                            }
+                            highest(s0);
+                            highest(s1);
+                            tmem_ld32(tS + ((i + 64) & 127), s0);  // at the end: the first columns again, for the second pass
+                            tmem_ld32(tS + ((i + 64) & 127) + 32, s1);
+                        }
+                    };
+                    if (whole) first_pass(Int<0>());
+                    else first_pass(Int<1>());
                     const float top = max_nan(mx[0], mx[1]) * a.scale_log2;
                     if (!(top < INFINITY)) l = NAN;  // a score that is NaN or +inf: so is the row's softmax
                     // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
@@ -732,9 +749,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                             if (lane == 0) mbar_arrive(&S.s_free[wg]);
                         }
                         uint32_t u0[16], u1[16];
-                        if (whole) {
+                        const unsigned bit = i == 0 ? 1u : 2u;
+                        if (!((part | none) & bit)) {
                             probabilities(s0, u0, Int<kPolyOf8>());
                             probabilities(s1, u1, Int<kPolyOf8>());
+                        } else if (none & bit) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) u0[j] = u1[j] = 0u;
                         } else {
                             hide(s0, i);
                             hide(s1, i + 32);
