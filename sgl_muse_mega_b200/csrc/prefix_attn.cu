@@ -1012,11 +1012,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 // ---- merge --------------------------------------------------------------------------------------------------------------
 // out = sum O_i 2^(m_i - M) / L over the pieces of the row's prefix item and own item, M = max m_i, L = sum l_i 2^(m_i - M). A
 // warp takes one row. Its lanes look up a candidate piece each (a CTA of the item's range, a part of its slot): which slot, m
-// and l, all requested at once; then D / 4 lanes read a piece's O (a float4 each), four loads in flight, in the order of the
+// and l, all requested at once; then D / 4 lanes read a piece's O (a float4 each), kAhead loads in flight, in the order of the
 // candidates. What rests on the lengths alone is done before the wait for the first kernel. The time is the chain of
 // three round trips to L2 (plan, m and l, O) behind that kernel's end.
-template <int D, bool kHalf>
-__global__ void __launch_bounds__(256, 3) prefix_merge_kernel(const __grid_constant__ PrefixAttnArgs a) {
+template <int D, bool kHalf, int kAhead>
+__global__ void __launch_bounds__(256, kAhead > 4 ? 2 : 3) prefix_merge_kernel(const __grid_constant__ PrefixAttnArgs a) {
     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;  // lanes of a piece, pieces read side by side
     const int lane = threadIdx.x & 31;
     const long long rows = (long long)a.rows * a.qh;
@@ -1085,7 +1085,6 @@ __global__ void __launch_bounds__(256, 3) prefix_merge_kernel(const __grid_const
             bool weighed = false;
             float g = 0.f;
             while (there != 0u) {  // O is asked for before m and l are looked at
-                constexpr int kAhead = 4;
                 float4 v[kAhead];
                 int from[kAhead];
 #pragma unroll
@@ -1135,6 +1134,10 @@ __global__ void __launch_bounds__(256, 3) prefix_merge_kernel(const __grid_const
     }
 }
 
+// Loads in flight of a merging thread where rows are so few that every block has its place at once: the rows' chains are what it
+// takes (64 decodes: 27.9 us with 4, 26.8 with 6, 8 or 10). Where blocks come in rounds, registers for a third block an SM do
+// more (32 x 16 rows: two blocks 125 us, three 121).
+constexpr int kWide = 8;
 template <int D, bool kHalf>
 static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const PrefixAttnMaps& maps, cudaStream_t s, bool pdl) {
     cudaLaunchAttribute attr[1];
@@ -1155,7 +1158,8 @@ static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const PrefixAttnMaps
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;  // its wait is its first statement, so it may always start under the first kernel's tail
-    return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf>, a);
+    if (blocks <= 2 * kCtas) return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf, kWide>, a);
+    return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf, 4>, a);
 }
 
 cudaError_t prefix_attn_launch(const PrefixAttnArgs& a, const PrefixAttnMaps& maps, int dim, bool fp16, cudaStream_t s, bool pdl) {
