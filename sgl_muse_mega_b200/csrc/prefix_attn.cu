@@ -20,10 +20,10 @@
 // rows, or gathers of four rows where pages are small or odd). Steps alternate between the two warpgroups, each with its
 // own S, P and O in tensor memory: while one takes the exponentials of its step the tensor core works for the other.
 //
-// Measured (whole launch, both kernels): 32 requests x 16 rows over 32 K shared tokens, 16 heads of 64 on 2 kv heads: 120 us = 579 TFLOP/s,
+// Measured (whole launch, both kernels): 32 requests x 16 rows over 32 K shared tokens, 16 heads of 64 on 2 kv heads: 121 us = 574 TFLOP/s,
 // bound by the softmax's phases that depend on one another (two steps a CTA take about 3000 cycles, their exponentials 2 x 900 of
-// those, their products 920); 96 requests over 2 K tokens of their own, 64 heads of 128 on 8: 157 us = 5.2 TB/s, DRAM and power;
-// 64 requests behind 8 K shared tokens 29 us, one request of 16 rows over a window of 2047 keys 20 us: latency.
+// those, their products 920); 96 requests over 2 K tokens of their own, 64 heads of 128 on 8: 154 us = 5.3 TB/s, DRAM and power;
+// 64 requests behind 8 K shared tokens 27 us, one request of 16 rows over a window of 2047 keys 18.6 us: latency.
 #include "batch.h"
 #include "umma.cuh"
 #include "util.cuh"
@@ -698,6 +698,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                             tmem_ld32(tS + ((i + 64) & 127) + 32, s1);
                         }
                     };
+                    // (a test of the mask inside the loop of whole tiles: 32 x 16 rows over 32 K tokens 123 us instead of 121)
                     if (whole) first_pass(Int<0>());
                     else first_pass(Int<1>());
                     const float top = max_nan(mx[0], mx[1]) * a.scale_log2;
