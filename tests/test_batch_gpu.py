@@ -318,6 +318,9 @@ ATTN = {
     "130 requests": dict(kv=[130 + i for i in range(130)], new=[1] * 130, prefix=128, qh=8, kvh=1, dim=64, page=128),
     "700 requests": dict(kv=[(37 * i) % 190 for i in range(700)], new=[min(i % 4, (37 * i) % 190) for i in range(700)], prefix=0, qh=8, kvh=2, dim=64,
                          page=16),
+    "halves of a tile": dict(kv=[63, 64, 65, 127, 128, 129, 191, 192, 193], new=[4, 4, 4, 4, 4, 4, 4, 4, 4], prefix=0, qh=8, kvh=1, dim=64, page=16),
+    "windows of half a tile": dict(kv=[200, 257, 320, 130], new=[16, 3, 1, 16], prefix=0, qh=8, kvh=1, dim=64, page=1, window=63),
+    "windows of half a tile, wide": dict(kv=[200, 257, 320, 130], new=[16, 3, 1, 16], prefix=64, qh=8, kvh=2, dim=128, page=8, window=64),
     "nothing behind the prefix": dict(kv=[256, 256, 256], new=[1, 4, 2], prefix=256, qh=8, kvh=1, dim=64, page=16),
     "128 heads a group": dict(kv=[200, 300], new=[2, 1], prefix=160, qh=128, kvh=1, dim=128, page=16),
     "256 heads a group": dict(kv=[200, 300], new=[2, 1], prefix=0, qh=256, kvh=1, dim=64, page=16),
