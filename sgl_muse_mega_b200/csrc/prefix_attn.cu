@@ -502,6 +502,13 @@ struct Int {
 };
 constexpr int kPolyOf8 = 1;
 
+// The probabilities p = 2^(score - m) are held as p 2^kLift, and l and O with them. f16 has no exponents below 2^-24: at 2^0 all keys of
+// less than 2^-25 of the largest one's weight left O and stayed in l (32 K keys of 2^-25.2 beside two of weight 1, in one CTA: 0 instead of
+// 4e-4, the two's V being 0).
+// At 2^7 the largest p is 2^(7 + 8) (m lags by up to 8), below f16's 65504; bf16 has f32's exponents.
+template <bool kHalf>
+constexpr float kLift = kHalf ? 7.f : 0.f;
+
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
@@ -705,7 +712,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     if (!(top < INFINITY)) l = NAN;  // a score that is NaN or +inf: so is the row's softmax
                     // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
                     // P's type and the f32 sums carry without loss), so O is seldom rescaled. (m = the maximum
-                    // where it moves: a key that carries the row has p = 1, which P's type holds exactly.)
+                    // where it moves: a key that carries the row has a power of two as its p, which P's type holds exactly.)
                     const bool grow = top > m + 8.f && rr < x.rows;
                     const bool any = __any_sync(0xffffffffu, grow);
                     const float mn = grow ? top : m, f = grow ? ex2(m - mn) : 1.f;  // m = -inf: the factor is 0
@@ -726,7 +733,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                         }
                     }
                     const float ms = m == -INFINITY ? 0.f : m;
-                    const float2 neg = make_float2(-ms, -ms);
+                    const float2 neg = make_float2(kLift<kHalf> - ms, kLift<kHalf> - ms);
                     float2 sum[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
@@ -1131,7 +1138,7 @@ __global__ void __launch_bounds__(256, kAhead > 4 ? 2 : 3) prefix_merge_kernel(c
         if (lane < kLanes)
             *(uint2*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * 4) * 2) =
                 make_uint2(pack2<kHalf>(o[0] * inv, o[1] * inv), pack2<kHalf>(o[2] * inv, o[3] * inv));
-        if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + log2f(Ls)) * kLn2;
+        if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + (log2f(Ls) - kLift<kHalf>)) * kLn2;
     }
 }
 

@@ -1,0 +1,107 @@
+"""The batched step's attention at the edges of what its rows see: keys in front of every window, infinite scores, scores far from
+zero, many keys of little weight, lengths that contradict the extents. Plain 64-bit forms: ``batch_ref.py``."""
+
+import math
+
+import pytest
+import torch
+
+import batch_ref as R
+from sgl_muse_mega_b200.common import host
+from sgl_muse_mega_b200.muse_spark.b200 import batch as BT
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+I32, I64, F32, BF, HF = torch.int32, torch.int64, torch.float32, torch.bfloat16, torch.float16
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def dev(x, dtype):
+    return torch.tensor(x, dtype=dtype, device=DEV)
+
+
+class Batch:
+    """`kv[b]` keys and `new[b]` rows a request; the whole pages of the first `prefix` keys are shared, the others lie in random
+    order, and the shared keys' values are the same in each request. The pool is finite everywhere."""
+
+    def __init__(self, seed, kv, new, prefix, qh, kvh, dim, page, dt, window=0, q_std=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.kv, self.new, self.prefix, self.page, self.window, self.dt = kv, new, prefix, page, window, dt
+        shared, pages = prefix // page, [-(-n // page) for n in kv]
+        total = shared + sum(max(p - shared, 0) for p in pages)
+        ids = torch.randperm(total, generator=g).tolist()
+        common, width = [ids.pop() for _ in range(shared)], max(pages)
+        rows = [common[: min(p, shared)] + [ids.pop() for _ in range(max(p - shared, 0))] for p in pages]
+        self.table = torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=I32)
+        self.k, self.v = (torch.randn(total * page, kvh, dim, generator=g).to(dt).to(DEV) for _ in range(2))
+        if prefix % page:
+            body = torch.randn(2, prefix % page, kvh, dim, generator=g).to(dt).to(DEV)
+            for b in range(len(kv)):
+                n = min(prefix, kv[b]) - shared * page
+                if n > 0:
+                    s = self.slots(b, range(shared * page, shared * page + n))
+                    self.k[s], self.v[s] = body[0, :n], body[1, :n]
+        self.cu = [0]
+        for n in new:
+            self.cu.append(self.cu[-1] + n)
+        self.q = (torch.randn(self.cu[-1], qh, dim, generator=g) * q_std).to(dt).to(DEV)
+
+    def slots(self, b, keys):
+        p = torch.tensor(list(keys))
+        return (self.table[b, p // self.page].long() * self.page + p % self.page).to(DEV)
+
+    def launch(self, **over):
+        lib = host.library()
+        self.lens = dict(block_table=self.table.to(DEV), kv_lens=dev(self.kv, I32), cu_rows=dev(self.cu, I32), prefix_len=dev([self.prefix], I32))
+        self.lens.update(over)
+        op = BT.PrefixAttention(lib, lib.load(), q=self.q, k_cache=self.k, v_cache=self.v, page_size=self.page, max_new=max(self.new),
+                                scale=0.125, window=self.window, lse=True, **self.lens)  # fmt: skip
+        op.out.fill_(5.0)
+        op.lse.fill_(5.0)
+        op.launch(stream())
+        torch.cuda.synchronize()
+        return op
+
+    def want(self):
+        return R.attention(self.q, self.k, self.v, self.table, self.kv, self.cu, self.page, 0.125, self.window)
+
+    def check(self, op, rows=slice(None)):
+        """The probabilities are rounded to the type once and the result once; f32 sums and the exponential are good to 1e-4 of the
+        weighted mean of |v| (scores of a few dozen: 2^-19 in the exponent, an exponential good to 4e-6). In f16 a probability has
+        a fixed step of 2^-24 below 2^-14; a row's largest is at least 2^7, so half such steps of all keys come to less than
+        keys x 2^-32 x 5."""
+        out, lse, mass = self.want()
+        eps = torch.finfo(self.dt).eps / 2
+        tol = out.abs() * eps + mass * (eps + 1e-4) + 1e-6 + (max(self.kv) * 2.0**-32 * 5 if self.dt == HF else 0.0)
+        err = (op.out.double().cpu() - out).abs()
+        assert (err <= tol)[rows].all(), float((err - tol)[rows].max())
+        assert ((op.lse.double().cpu() - lse).abs() <= 1e-4 + lse.abs() * 2.0**-22)[rows].all()
+
+
+# ---- many keys of little weight ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_many_keys_of_little_weight(dt):
+    """Two keys of weight 1 beside 32,766 of 2^-25.2 each, 4e-4 of the row together, by one CTA: they stay in the result."""
+    n, B, page = 32768, 160, 128
+    k, v = torch.zeros(n, 1, 64, dtype=dt, device=DEV), torch.ones(n, 1, 64, dtype=dt, device=DEV)
+    k[..., 0] = -140.0  # a score of -17.5
+    for one in (3, 200):  # a tile of each parity
+        k[one], v[one] = 0.0, 0.0
+    q = torch.zeros(B, 1, 64, dtype=dt, device=DEV)
+    q[..., 0] = 1.0
+    table = torch.arange(n // page, dtype=I32, device=DEV).repeat(B, 1)
+    lib = host.library()
+    op = BT.PrefixAttention(lib, lib.load(), q=q, k_cache=k, v_cache=v, block_table=table, kv_lens=dev([n] * B, I32),
+                            cu_rows=dev(list(range(B + 1)), I32), prefix_len=dev([0], I32), page_size=page, max_new=1, scale=0.125, lse=True)  # fmt: skip
+    op.launch(stream())
+    torch.cuda.synchronize()
+    low = (n - 2) * math.exp(-17.5)
+    out = low / (2 + low)
+    # a probability's rounding (f16: half a step of 2^-24 of the 2^7 that the largest is held at, over a sum of 2), the result's (f16 has a
+    # step of 2^-24 here too); the exponential 4e-6, f32 sums of 32 K values 2^-17
+    step = n * 2.0**-33 + 2.0**-25 if dt == HF else out * 2.0**-9
+    assert ((op.out.double() - out).abs() <= out * (torch.finfo(dt).eps / 2 + 2.0**-16) + step).all()
+    assert ((op.lse.double() - math.log(2 + low)).abs() <= 2.0**-16).all()
