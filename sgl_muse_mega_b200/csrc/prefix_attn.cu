@@ -93,7 +93,8 @@ __device__ __forceinline__ void tiles_of(unsigned lo, unsigned hi, unsigned lead
 
 struct Plan {
     int prefix;         // shared keys (0: none shared)
-    int p_lo;           // first shared key that any row sees
+    int first;          // first shared key that any row sees
+    int p_lo;           // where tile 0 of the prefix items starts: a multiple of kTile
     int ref;            // the request whose table row names the shared pages
     int tokens;         // rows of the batch
     unsigned tiles;     // key tiles of a prefix item
@@ -187,7 +188,8 @@ __device__ __forceinline__ Plan make_plan(const PrefixAttnArgs& a, const Lens& l
     // one request shares with nobody, and a prefix that no request holds whole cannot be read through one table row
     p.prefix = live > 1 && ref != 0x7fffffff ? want : 0;
     p.ref = p.prefix > 0 ? ref : 0;
-    p.p_lo = p.prefix > 0 ? lo / kTile * kTile : 0;
+    p.first = p.prefix > 0 ? lo : 0;
+    p.p_lo = p.first / kTile * kTile;
     p.tiles = p.prefix > 0 && hi > p.p_lo ? (unsigned)(hi - p.p_lo + kTile - 1) / kTile : 0u;
     p.per_head = head_steps(a, p.tiles, p.tokens * a.G);
     p.prefix_steps = p.per_head * a.kvh;
@@ -243,6 +245,7 @@ struct Piece {
     int n;            // request rows (own items)
     int first, len;   // the request's first row and keys
     int key0;         // first key of the item's tile 0
+    int seen;         // first key that any of its rows sees: those in front are not read
     unsigned t0, t1;  // key tiles [t0, t1)
     __device__ __forceinline__ bool pair() const { return rows > kTile; }
     __device__ __forceinline__ unsigned steps() const { return (t1 - t0) << (rows > kTile ? 1 : 0); }
@@ -259,7 +262,7 @@ struct Walker {
     unsigned off;   // steps of it that lie before the range
     Req r;
     unsigned tiles;
-    int row_total, blocks, key0;
+    int row_total, blocks, key0, seen;
 
     __device__ __forceinline__ Walker(const PrefixAttnArgs& a_, const Plan& p_, const Lens& lens, int cta, int lane) : a(a_), p(p_) {
         unsigned pos = range_lo(p.total, cta);
@@ -303,10 +306,12 @@ struct Walker {
             tiles = p.tiles;
             r = Req{0, p.tokens, p.prefix};
             key0 = p.p_lo;
+            seen = p.first;
         } else {
             r = request(a, b);
             tiles = own_tiles(a, r, p.prefix);
             key0 = own_start(a, r, p.prefix);
+            seen = own_first(a, r, p.prefix);
         }
         row_total = r.n * a.G;
         blocks = row_blocks(row_total);
@@ -331,6 +336,7 @@ struct Walker {
             x.n = r.n;
             x.len = r.len;
             x.key0 = key0;
+            x.seen = seen;
             x.index = (b < 0 ? 0 : items) + h * blocks + rb;
             const int sh = x.rows > kTile ? 1 : 0;
             const unsigned front = lead(a, sh != 0), len = (tiles << sh) + front, stop = min(off + left, len);
@@ -900,8 +906,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     } else {
         // ---- queries and K rows (warp 9), V rows (warp 10) ----
         // Where pages hold runs of 8 or more aligned rows, a lane copies a run as one box; else a lane gathers four rows. Rows
-        // past the piece's last key are asked for behind the pool's end, which reads zeros: a probability of zero times
-        // whatever a stale row holds would not be zero. So the run that the last key ends in is gathered row by row (V).
+        // in front of the first key that any of the piece's rows sees and past its last one are asked for behind the pool's end,
+        // which reads zeros: a probability of zero times whatever a stale row holds would not be zero. So the runs that the first
+        // and the last key lie in are gathered row by row (V), and page ids outside [first, last] are not looked at.
         const bool is_v = warp == 10;
         const CUtensorMap *run_map = is_v ? &maps.v_run : &maps.k_run, *row_map = is_v ? &maps.v_row : &maps.k_row;
         unsigned char* ring = is_v ? Vs : Ks;
@@ -916,7 +923,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             const int* trow = a.table + (long long)(x.b < 0 ? p.ref : x.b) * a.table_row;
             const int stop = min(x.len, cap), col = x.h * head;
             auto slot_of = [&](int k, int n) -> int {  // pool row of key k, of n rows that lie in one page
-                if (k >= stop) return a.kv_rows;
+                if (k >= stop || k + n <= x.seen) return a.kv_rows;
                 const int pg = a.page_shift >= 0 ? k >> a.page_shift : k / a.page;
                 const long long slot = (long long)__ldg(trow + pg) * a.page + (k - pg * a.page);
                 if (slot >= 0 && slot + n <= a.kv_rows) return (int)slot;
@@ -977,11 +984,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
                         for (int c = 0; c < C::kAtoms; ++c)
                             gather4(dst + c * (kTile * 128), row_map, col + 64 * c, y[0], y[1], y[2], y[3], &full[i]);
-                    } else if (is_v && k < stop && k + per > stop) {
+                    } else if (is_v && ((k < stop && k + per > stop) || (k < x.seen && k + per > x.seen))) {
                         for (int j = 0; j < per; j += 4) {
                             int z[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) z[e] = y[0] < a.kv_rows && k + j + e < stop ? y[0] + j + e : a.kv_rows;
+                            for (int e = 0; e < 4; ++e) {
+                                const int key = k + j + e;
+                                z[e] = y[0] < a.kv_rows && key >= x.seen && key < stop ? y[0] + j + e : a.kv_rows;
+                            }
 #pragma unroll
                             for (int c = 0; c < C::kAtoms; ++c)
                                 gather4(dst + c * (kTile * 128) + j * 128, row_map, col + 64 * c, z[0], z[1], z[2], z[3], &full[i]);

@@ -105,3 +105,40 @@ def test_many_keys_of_little_weight(dt):
     step = n * 2.0**-33 + 2.0**-25 if dt == HF else out * 2.0**-9
     assert ((op.out.double() - out).abs() <= out * (torch.finfo(dt).eps / 2 + 2.0**-16) + step).all()
     assert ((op.lse.double() - math.log(2 + low)).abs() <= 2.0**-16).all()
+
+
+# ---- keys in front of every window ------------------------------------------------------------------------------------
+FRONT = {
+    "inside the prefix": dict(kv=[700, 705, 760], new=[2, 1, 3], prefix=640, window=100),  # first key that a row sees: 598
+    "inside the prefix, more rows than a block": dict(kv=[700, 705, 760], new=[40, 1, 3], prefix=640, window=90),
+    "behind the prefix": dict(kv=[700, 900], new=[2, 1], prefix=300, window=77),
+    "alone": dict(kv=[700], new=[16], prefix=0, window=127),
+    "no prefix": dict(kv=[700, 431, 90], new=[3, 1, 2], prefix=0, window=50),
+}
+
+
+@pytest.mark.parametrize("dt,dim", [(BF, 64), (HF, 64), (BF, 128)])
+@pytest.mark.parametrize("page", [1, 7, 8, 16, 24, 128])
+@pytest.mark.parametrize("name", list(FRONT))
+def test_keys_in_front_of_every_window(name, page, dt, dim):
+    """Rows that no window reaches are not read: NaN and infinities there change nothing, neither do page ids outside the pool for
+    pages that have slid out of every window."""
+    c = Batch(page, qh=8, kvh=1, dim=dim, page=page, dt=dt, **FRONT[name])
+    firsts = [max(0, n - m - c.window) for n, m in zip(c.kv, c.new)]
+    low = min(firsts)
+    for b, n in enumerate(c.kv):
+        gone = [k for k in range(n) if k < low or c.prefix <= k < firsts[b]]
+        if gone:
+            s = c.slots(b, gone)
+            c.k[s], c.v[s] = math.nan, math.nan
+            c.v[s[::2]] = math.inf
+    clean = c.table.clone()
+    for b in range(len(c.kv)):
+        for p in range(clean.shape[1]):
+            last = (p + 1) * page - 1  # the page's last key
+            if last < low or (p * page >= c.prefix and last < firsts[b]):
+                c.table[b, p] = -1 if p % 2 else 1 << 30
+    op = c.launch()
+    assert op.status[0].item() == 0
+    c.table = clean
+    c.check(op)
