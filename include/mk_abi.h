@@ -780,12 +780,12 @@ int mk_rotary_bind(MkModule* module, const MkRotaryBind* bind, MkLaunch** out);
 // Attention of a batch's new rows over the paged cache. Request b's rows are [cu_rows[b], cu_rows[b + 1]), the last of its
 // kv_lens[b] keys; its row at position x sees the keys max(0, x - window) .. x (window 0: all up to x). The first prefix_len keys
 // are the same cache rows for every request (their block-table rows begin alike) and are read once for the whole batch; a
-// request shorter than that sees its own length of them. A row that sees no key is 0 with lse -inf. Softmax statistics and sums
-// are f32; the probabilities are rounded to the inputs' type for the product with V. Of the prefix the keys from the first that any
-// row of the batch sees are read, behind it those from the first that any of the request's rows sees up to kv_lens[b]: what lies
-// elsewhere in the pool has no part in a result, and table entries of pages that lie wholly in front may hold anything. Within
-// those keys a NaN or infinity in a V row may reach rows that do not see its key (0 x NaN in the product); in a K row it
-// reaches the rows that see it. Page ids outside the pool are recorded (code 4) and read as zero rows.
+// request shorter than that sees its own length of them. A row that sees no key, or only keys whose scores are -inf, is 0 with lse
+// -inf. Softmax statistics and sums are f32; the probabilities are rounded to the inputs' type for the product with V. Of the prefix
+// the keys from the first that any row of the batch sees are read, behind it those from the first that any of the request's rows
+// sees up to kv_lens[b]: what lies elsewhere in the pool has no part in a result, and table entries of pages that lie wholly in
+// front may hold anything. Within those keys a NaN or infinity in a V row may reach rows that do not see its key (0 x NaN in the
+// product); in a K row it reaches the rows that see it. Page ids outside the pool are recorded (code 4) and read as zero rows.
 typedef struct MkPrefixAttnBind {
     uint64_t q;            // bf16 or f16 [rows, q_heads, head_dim]
     int64_t q_row;         // strides in elements, multiples of 8

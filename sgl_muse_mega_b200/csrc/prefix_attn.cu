@@ -487,13 +487,14 @@ __device__ __forceinline__ float max_nan(float x, float y, float z) {
     return r;
 }
 // 2^x for two x on the FMA pipe: x = k + f with k the nearest whole number, 2^f on [-1/2, 1/2] by the polynomial of degree 4 with
-// p(0) = 1 and the least relative error (2.9e-6; a linear program), k added to the exponent. x is kept at or above -126. The
-// special-function unit yields 16 results a clock and SM; kPolyOf8 of 8 results come from here instead, except in tiles with masked
-// keys, whose probabilities have to be exactly 0. (0 of 8: 128.5 us for the 32 x 16 rows over 32 K tokens, 1: 125, 2: 125.5, 3: 129.)
+// p(0) = 1 and the least relative error (2.9e-6; a linear program), k added to the exponent. x is kept at or above -127, whose result is
+// exactly 0 (p = 1 with its exponent's 127 taken off), so a score of -inf weighs nothing; between -127 and -126 it is some number below 2^-126.
+// The special-function unit yields 16 results a clock and SM; kPolyOf8 of 8 results come from here instead, except in the few tiles with
+// masked keys. (0 of 8: 128.5 us for the 32 x 16 rows over 32 K tokens, 1: 125, 2: 125.5, 3: 129.)
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
     const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
+    x.x = fmaxf(x.x, -127.f);
+    x.y = fmaxf(x.y, -127.f);
     const float2 r = add2(x, magic);  // k in the low bits
     const float2 f = fma2(add2(r, back), make_float2(-1.f, -1.f), x);
     float2 p = fma2(f, make_float2(0x1.3a007ap-7f, 0x1.3a007ap-7f), make_float2(0x1.c9fd1ep-5f, 0x1.c9fd1ep-5f));

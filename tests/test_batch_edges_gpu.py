@@ -142,3 +142,26 @@ def test_keys_in_front_of_every_window(name, page, dt, dim):
     assert op.status[0].item() == 0
     c.table = clean
     c.check(op)
+
+
+# ---- scores of -inf ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("dim,page", [(64, 16), (64, 1), (128, 64)])
+def test_scores_of_minus_infinity(dt, dim, page):
+    """A key whose score is -inf has weight 0, whatever its V row holds; a row that has only such keys is 0 with lse -inf."""
+    c = Batch(3, kv=[700, 640, 650], new=[2, 1, 2], prefix=384, qh=8, kvh=1, dim=dim, page=page, dt=dt)
+    c.q[:, :, 0] = 1.0
+    big = torch.finfo(dt).max
+    for b, keys in ((0, [5, 200, 383, 384, 500]), (2, range(384, 600))):  # shared and own ones; whole tiles of request 2
+        s = c.slots(b, keys)
+        c.k[s, :, 0], c.v[s] = -math.inf, big
+    op = c.launch()
+    c.check(op)
+    for b in range(3):  # and now all of them, in tiles that nothing masks
+        c.k[c.slots(b, range(c.kv[b])), :, 0] = -math.inf
+    c.k[c.slots(1, [639]), :, 0] = 0.0  # the one key that request 1's row keeps
+    op = c.launch()
+    out, lse = op.out.double().cpu(), op.lse.double().cpu()
+    for r in (0, 1, 3, 4):
+        assert (out[r] == 0).all() and (lse[r] == -math.inf).all(), r
+    assert torch.equal(op.out[2], c.v[c.slots(1, [639])][0].expand(8, dim)) and op.status[0].item() == 0
