@@ -515,6 +515,10 @@ constexpr int kPolyOf8 = 1;
 // At 2^7 the largest p is 2^(7 + 8) (m lags by up to 8), below f16's 65504; bf16 has f32's exponents.
 template <bool kHalf>
 constexpr float kLift = kHalf ? 7.f : 0.f;
+// From here on (in the exponent) the differences of scores are taken before they are scaled; below, the reference is rounded by at most
+// 2^-15, which is what the pieces of a row may differ by. The test for it costs a vote a step (verify 121.8 -> 123.8 us, 64 decodes
+// 27.7 -> 28.3); a vote only where the reference moves, a loop of its own for such scores, or one vote for this and the rescaling cost more.
+constexpr float kFar = 1024.f;
 
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -715,15 +719,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                     // (a test of the mask inside the loop of whole tiles: 32 x 16 rows over 32 K tokens 123 us instead of 121)
                     if (whole) first_pass(Int<0>());
                     else first_pass(Int<1>());
-                    const float top = max_nan(mx[0], mx[1]) * a.scale_log2;
+                    const float top = max_nan(mx[0], mx[1]);
                     if (!(top < INFINITY)) l = NAN;  // a score that is NaN or +inf: so is the row's softmax
-                    // The reference exponent m follows the maximum only when it has grown by more than 8 (a factor 256 that
+                    // The reference score m (not scaled) follows the maximum only when that has grown by more than 2^8 (a factor that
                     // P's type and the f32 sums carry without loss), so O is seldom rescaled. (m = the maximum
                     // where it moves: a key that carries the row has a power of two as its p, which P's type holds exactly.)
-                    const bool grow = top > m + 8.f && rr < x.rows;
+                    const bool grow = (top - m) * a.scale_log2 > 8.f && rr < x.rows;
                     const bool any = __any_sync(0xffffffffu, grow);
-                    const float mn = grow ? top : m, f = grow ? ex2(m - mn) : 1.f;  // m = -inf: the factor is 0
-                    m = mn;
+                    const float f = grow ? ex2((m - top) * a.scale_log2) : 1.f;  // m = -inf: the factor is 0
+                    if (grow) m = top;
                     l *= f;
                     // the P V product of this warpgroup's last step has read P and updated O
                     if (!C::kAlias && !(ok = attn_wait(&S.pv_done[wg], pv_par, &S, a.status, 540))) break;
@@ -739,8 +743,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                             tmem_st16(tO + i, o);
                         }
                     }
-                    const float ms = m == -INFINITY ? 0.f : m;
-                    const float2 neg = make_float2(kLift<kHalf> - ms, kLift<kHalf> - ms);
+                    // Exponents are scale s - scale m in one FMA, whose second term is rounded. All weights of a row have the same
+                    // factor from that, so it is of no account until its half step passes the exponents that P's type can carry
+                    // (2^27 and up with f16: NaN). Where it counts the differences s - m are taken first.
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    const bool far = __any_sync(0xffffffffu, fabsf(ref * a.scale_log2) >= kFar);
+                    const float shift = far ? kLift<kHalf> : kLift<kHalf> - ref * a.scale_log2;
+                    const float2 neg = make_float2(shift, shift);
+                    const unsigned slow = part | none | (far ? 3u : 0u);  // halves that are masked, or whose scores are far from zero
                     float2 sum[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
@@ -765,13 +775,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                         }
                         uint32_t u0[16], u1[16];
                         const unsigned bit = i == 0 ? 1u : 2u;
-                        if (!((part | none) & bit)) {
+                        if (!(slow & bit)) {
                             probabilities(s0, u0, Int<kPolyOf8>());
                             probabilities(s1, u1, Int<kPolyOf8>());
                         } else if (none & bit) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) u0[j] = u1[j] = 0u;
                         } else {
+                            if (far) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) s0[j] -= ref, s1[j] -= ref;
+                            }
                             hide(s0, i);
                             hide(s1, i + 32);
                             probabilities(s0, u0, Int<0>());
@@ -1029,7 +1043,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 }
 
 // ---- merge --------------------------------------------------------------------------------------------------------------
-// out = sum O_i 2^(m_i - M) / L over the pieces of the row's prefix item and own item, M = max m_i, L = sum l_i 2^(m_i - M). A
+// out = sum O_i w_i / L over the pieces of the row's prefix item and own item, w_i = 2^(scale (m_i - M)), M = max m_i, L = sum l_i w_i. A
 // warp takes one row. Its lanes look up a candidate piece each (a CTA of the item's range, a part of its slot): which slot, m
 // and l, all requested at once; then D / 4 lanes read a piece's O (a float4 each), kAhead loads in flight, in the order of the
 // candidates. What rests on the lengths alone is done before the wait for the first kernel. The time is the chain of
@@ -1122,8 +1136,8 @@ __global__ void __launch_bounds__(256, kAhead > 4 ? 2 : 3) prefix_merge_kernel(c
                 if (!weighed) {
                     weighed = true;
                     const float mn = fmaxf(M, warp_max(m));
-                    const float f = M == mn ? 1.f : ex2(M - mn);   // of what is there
-                    g = l == 0.f ? 0.f : m == mn ? 1.f : ex2(m - mn);  // of this lane's piece (l is NaN where a score was)
+                    const float f = M == mn ? 1.f : ex2((M - mn) * a.scale_log2);           // of what is there
+                    g = l == 0.f ? 0.f : m == mn ? 1.f : ex2((m - mn) * a.scale_log2);  // of this lane's piece (l is NaN where a score was)
                     M = mn;
                     Ls = Ls * f + warp_sum(l * g);
 #pragma unroll
@@ -1149,7 +1163,7 @@ __global__ void __launch_bounds__(256, kAhead > 4 ? 2 : 3) prefix_merge_kernel(c
         if (lane < kLanes)
             *(uint2*)((unsigned char*)a.out + ((long long)tok * a.o_row + head * a.o_head + lane * 4) * 2) =
                 make_uint2(pack2<kHalf>(o[0] * inv, o[1] * inv), pack2<kHalf>(o[2] * inv, o[3] * inv));
-        if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M + (log2f(Ls) - kLift<kHalf>)) * kLn2;
+        if (a.lse != nullptr && lane == 0) a.lse[(long long)tok * a.qh + head] = Ls == 0.f ? -INFINITY : (M * a.scale_log2 + (log2f(Ls) - kLift<kHalf>)) * kLn2;
     }
 }
 

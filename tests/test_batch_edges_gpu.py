@@ -165,3 +165,25 @@ def test_scores_of_minus_infinity(dt, dim, page):
     for r in (0, 1, 3, 4):
         assert (out[r] == 0).all() and (lse[r] == -math.inf).all(), r
     assert torch.equal(op.out[2], c.v[c.slots(1, [639])][0].expand(8, dim)) and op.status[0].item() == 0
+
+
+# ---- scores far from zero ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt,length,step", [(BF, 2.0**8, 8.0), (HF, 2.0**8, 8.0), (BF, 2.0**11, 64.0), (HF, 2.0**11, 64.0), (BF, 2.0**15, 512.0),
+                                            (HF, 2.0**15, 512.0), (BF, 2.0**30, 2.0**40)])  # fmt: skip
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_far_from_zero(dt, length, step, sign, dim):
+    """Only the scores' differences count: up to 3 length^2 / 8 with steps of `step` / 8 between the keys, all of them exact in f32.
+    Some references are large enough that a rounded one would be off by more than f16's or f32's exponents."""
+    c = Batch(7, kv=[900, 800, 555], new=[2, 1, 3], prefix=512, qh=8, kvh=1, dim=dim, page=16, dt=dt)
+    g = torch.Generator().manual_seed(int(math.log2(length)))
+    c.q.zero_()
+    c.k.zero_()
+    c.q[..., :3] = (length * (1 - torch.arange(8) / 32.0))[None, :, None].to(dt).to(DEV)  # a length of its own for each head
+    c.q[..., 3] = math.sqrt(step) if step > 2.0**16 else 1.0
+    c.k[..., :3] = sign * length
+    level = torch.randint(-8, 9, c.k.shape[:2], generator=g).to(DEV)
+    c.k[..., 3] = (level * (step / c.q[0, 0, 3].double())).to(dt)
+    op = c.launch()
+    assert torch.isfinite(op.out).all() and op.status[0].item() == 0
+    c.check(op)
