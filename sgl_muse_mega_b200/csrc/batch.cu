@@ -35,7 +35,7 @@ __device__ __forceinline__ TablesShared tables_carve(unsigned char* p, int batch
     s.twice = s.seen + words;
     return s;
 }
-size_t block_tables_smem(int batch, int pool_rows) { return ((size_t)batch * 6 + 1) * 4 + (size_t)((pool_rows + 31) / 32) * 8; }
+static size_t block_tables_smem(int batch, int pool_rows) { return ((size_t)batch * 6 + 1) * 4 + (size_t)((pool_rows + 31) / 32) * 8; }
 
 constexpr int kTablesThreads = 256;
 
@@ -380,45 +380,54 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 template <typename K, typename A>
-static cudaError_t launch_batch(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl, const A& a) {
+static cudaError_t launch_batch(K kern, const BatchDims& d, cudaStream_t s, bool pdl, const A& a) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(d.grid);
+    cfg.blockDim = dim3(d.block);
+    cfg.dynamicSmemBytes = d.smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-cudaError_t block_tables_launch(const BlockTablesArgs& a, int sms, cudaStream_t s, bool pdl) {
+BatchDims block_tables_dims(const BlockTablesArgs& a, int sms) {
     const long long chunks = (long long)a.batch * ((a.width + 1023) / 1024), rows = ((long long)a.rows + kTablesThreads - 1) / kTablesThreads;
     long long grid = chunks > rows ? chunks : rows;
     if (grid > 2 * sms) grid = 2 * sms;
-    return launch_batch(block_tables_kernel, dim3((unsigned)grid), dim3(kTablesThreads), block_tables_smem(a.batch, a.pool_rows), s, pdl, a);
+    return {(unsigned)grid, kTablesThreads, block_tables_smem(a.batch, a.pool_rows)};
+}
+cudaError_t block_tables_launch(const BlockTablesArgs& a, int sms, cudaStream_t s, bool pdl) {
+    return launch_batch(block_tables_kernel, block_tables_dims(a, sms), s, pdl, a);
 }
 
+// 16 positions a thread once that fills the SMs; 4 for short tables, whose time is one thread's chain
+static int rope_rows(const RopeTableArgs& a, int sms) { return (a.rows + 15) / 16 * (a.rot / 8) >= 256ll * sms ? 16 : 4; }
+BatchDims rope_table_dims(const RopeTableArgs& a, int sms) {
+    const long long rows = rope_rows(a, sms), groups = a.rot / 8;
+    return {(unsigned)(((a.rows + rows - 1) / rows * groups + 127) / 128), 128, 0};
+}
 cudaError_t rope_table_launch(const RopeTableArgs& a, int sms, cudaStream_t s, bool pdl) {
-    const long long groups = a.rot / 8;
-    auto grid = [&](int rows) { return dim3((unsigned)(((a.rows + rows - 1) / rows * groups + 127) / 128)); };
-    // 16 positions a thread once that fills the SMs; 4 for short tables, whose time is one thread's chain
-    if ((a.rows + 15) / 16 * groups >= 256ll * sms) return launch_batch(rope_table_kernel<16>, grid(16), dim3(128), 0, s, pdl, a);
-    return launch_batch(rope_table_kernel<4>, grid(4), dim3(128), 0, s, pdl, a);
+    if (rope_rows(a, sms) == 16) return launch_batch(rope_table_kernel<16>, rope_table_dims(a, sms), s, pdl, a);
+    return launch_batch(rope_table_kernel<4>, rope_table_dims(a, sms), s, pdl, a);
 }
 
-template <typename T>
-static cudaError_t rotary_typed(const RotaryArgs& a, bool inter, cudaStream_t s, bool pdl) {
-    const bool wide = inter || (a.rot / 2) % 8 == 0;
-    const int n = wide ? 8 : 4, pieces = (inter ? a.rot / n : a.rot / 2 / n) + (a.dim - a.rot) / n;
+static bool rotary_wide(const RotaryArgs& a, bool inter) { return inter || (a.rot / 2) % 8 == 0; }
+BatchDims rotary_dims(const RotaryArgs& a, bool inter) {
+    const int n = rotary_wide(a, inter) ? 8 : 4, pieces = (inter ? a.rot / n : a.rot / 2 / n) + (a.dim - a.rot) / n;
     int threads = ((a.qh + a.kvh) * pieces + 31) / 32 * 32;
     if (threads > 256) threads = 256;
-    const dim3 grid((unsigned)a.rows), block((unsigned)threads);
-    if (inter) return launch_batch(rotary_kernel<T, 8, true>, grid, block, 0, s, pdl, a);
-    if (wide) return launch_batch(rotary_kernel<T, 8, false>, grid, block, 0, s, pdl, a);
-    return launch_batch(rotary_kernel<T, 4, false>, grid, block, 0, s, pdl, a);
+    return {(unsigned)a.rows, (unsigned)threads, 0};
+}
+template <typename T>
+static cudaError_t rotary_typed(const RotaryArgs& a, bool inter, cudaStream_t s, bool pdl) {
+    const BatchDims d = rotary_dims(a, inter);
+    if (inter) return launch_batch(rotary_kernel<T, 8, true>, d, s, pdl, a);
+    if (rotary_wide(a, inter)) return launch_batch(rotary_kernel<T, 8, false>, d, s, pdl, a);
+    return launch_batch(rotary_kernel<T, 4, false>, d, s, pdl, a);
 }
 cudaError_t rotary_launch(const RotaryArgs& a, bool fp16, bool interleaved, cudaStream_t s, bool pdl) {
     return fp16 ? rotary_typed<__half>(a, interleaved, s, pdl) : rotary_typed<__nv_bfloat16>(a, interleaved, s, pdl);

@@ -101,11 +101,20 @@ struct PrefixAttnMaps {
     CUtensorMap k_run, v_run, k_row, v_row, q;
 };
 
+// a kernel's launch shape
+struct BatchDims {
+    unsigned grid, block;
+    size_t smem;
+};
+BatchDims block_tables_dims(const BlockTablesArgs& a, int sms);
+BatchDims rope_table_dims(const RopeTableArgs& a, int sms);
+BatchDims rotary_dims(const RotaryArgs& a, bool interleaved);
+BatchDims prefix_attn_dims(int dim);                        // its first kernel
+BatchDims prefix_merge_dims(const PrefixAttnArgs& a);       // its second
 cudaError_t block_tables_launch(const BlockTablesArgs& a, int sms, cudaStream_t s, bool pdl);
 cudaError_t rope_table_launch(const RopeTableArgs& a, int sms, cudaStream_t s, bool pdl);
 cudaError_t rotary_launch(const RotaryArgs& a, bool fp16, bool interleaved, cudaStream_t s, bool pdl);
 cudaError_t prefix_attn_launch(const PrefixAttnArgs& a, const PrefixAttnMaps& maps, int dim, bool fp16, cudaStream_t s, bool pdl);
-size_t block_tables_smem(int batch, int pool_rows);
 cudaError_t batch_prepare();
 cudaError_t prefix_attn_prepare();
 

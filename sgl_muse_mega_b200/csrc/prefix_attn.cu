@@ -1171,27 +1171,32 @@ __global__ void __launch_bounds__(256, kAhead > 4 ? 2 : 3) prefix_merge_kernel(c
 // takes (64 decodes: 27.9 us with 4, 26.8 with 6, 8 or 10). Where blocks come in rounds, registers for a third block an SM do
 // more (32 x 16 rows: two blocks 125 us, three 121).
 constexpr int kWide = 8;
+BatchDims prefix_attn_dims(int dim) { return {kCtas, kAttnThreads, (size_t)(dim == 64 ? Cfg<64>::kSmem : Cfg<128>::kSmem)}; }
+BatchDims prefix_merge_dims(const PrefixAttnArgs& a) {
+    // at most four rounds of three blocks an SM: rows beyond the batch's must not cost a block each
+    const long long blocks = ((long long)a.rows * a.qh + 7) / 8, most = 12ll * kCtas;
+    return {(unsigned)(blocks < most ? blocks : most), 256, 0};
+}
 template <int D, bool kHalf>
 static cudaError_t prefix_attn_run(const PrefixAttnArgs& a, const PrefixAttnMaps& maps, cudaStream_t s, bool pdl) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kCtas);
-    cfg.blockDim = dim3(kAttnThreads);
-    cfg.dynamicSmemBytes = Cfg<D>::kSmem;
+    const BatchDims d = prefix_attn_dims(D), merge = prefix_merge_dims(a);
+    cfg.gridDim = dim3(d.grid);
+    cfg.blockDim = dim3(d.block);
+    cfg.dynamicSmemBytes = d.smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
     cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_attn_kernel<D, kHalf>, a, maps);
     if (e != cudaSuccess) return e;
-    // at most four rounds of three blocks an SM: rows beyond the batch's must not cost a block each
-    const long long blocks = ((long long)a.rows * a.qh + 7) / 8, most = 12ll * kCtas;
-    cfg.gridDim = dim3((unsigned)(blocks < most ? blocks : most));
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
+    cfg.gridDim = dim3(merge.grid);
+    cfg.blockDim = dim3(merge.block);
+    cfg.dynamicSmemBytes = merge.smem;
     cfg.numAttrs = 1;  // its wait is its first statement, so it may always start under the first kernel's tail
-    if (blocks <= 2 * kCtas) return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf, kWide>, a);
+    if (merge.grid <= 2 * kCtas) return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf, kWide>, a);
     return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<D, kHalf, 4>, a);
 }
 

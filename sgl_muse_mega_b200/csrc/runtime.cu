@@ -1081,9 +1081,20 @@ int mk_launch_info(const MkLaunch* launch, MkLaunchInfo* out) {
         out->cluster = 1;
         out->grid = L->op_kind[0] == OP_GEMM_BF16 ? gemm_grid(L->op_gemm) : 16;
         out->smem = L->op_kind[0] == OP_GEMM_BF16 ? (int64_t)gemm_smem(L->op_gemm, false) : 0;
+        const BatchDims batch = L->op_kind[0] == OP_BLOCK_TABLES ? block_tables_dims(L->tables, L->sms)
+                                : L->op_kind[0] == OP_ROPE_TABLE ? rope_table_dims(L->rope_table, L->sms)
+                                : L->op_kind[0] == OP_ROTARY     ? rotary_dims(L->rotary, L->interleaved)
+                                : L->op_kind[0] == OP_PREFIX_ATTN ? prefix_attn_dims(L->head_dim)
+                                                                 : BatchDims{0, 0, 0};
+        if (batch.grid > 0) {
+            out->grid = batch.grid;
+            out->block = batch.block;
+            out->smem = (int64_t)batch.smem;
+        }
         if (L->op_kind[0] == OP_PREFIX_ATTN) {
+            const BatchDims merge = prefix_merge_dims(L->pattn);
             out->kernels = 2;
-            out->grid = kAttnCtas;
+            if (merge.grid > batch.grid) out->grid = merge.grid;
         }
         out->param_bytes = (int64_t)sizeof(MkLaunch);
         return 0;
