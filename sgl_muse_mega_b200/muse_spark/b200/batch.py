@@ -6,7 +6,8 @@ rows of a ``RopeTable``, append of k and v at the slots) and ``PrefixAttention``
 prefix that all requests share visited once). Each class owns its outputs and scratch, binds once, and ``launch(stream, pdl)``
 enqueues it (graph-capturable: lengths are read on the device). A bound object may not overlap itself on two streams.
 
-``status`` of each (i32 [16]) stays 0 until a launch leaves something out; ``include/mk_abi.h`` lists what.
+``status`` (i32 [16]; ``RopeTable`` has nothing to leave out) stays 0 until a launch leaves something out;
+``include/mk_abi.h`` lists what.
 """
 
 from __future__ import annotations
@@ -130,8 +131,9 @@ class Rotary:
         """``q`` / ``k`` / ``v``: bf16 or f16 [rows, heads, dim], rows and heads may be strided (slices of a fused
         projection). ``cos_sin_cache`` f32 [positions, rot]: its width is the number of rotated dims. ``slots`` i64 [rows]:
         pool rows (negative: not appended). ``q_out``: a new tensor unless given; ``q_out=q`` / ``k_out=k`` rotate in
-        place. ``n_rows`` i32 [1] on the device: live rows (the rest is left as it was). ``inverse`` rotates back, which is
-        also the rotation's gradient."""
+        place. ``n_rows`` i32 [1] on the device: live rows (the rest is left as it was). ``interleaved``: neighbouring pairs
+        (the target's heads), else the two halves of the rotated dims (the draft's). ``inverse`` rotates back, which is also the
+        rotation's gradient."""
         dev, dt = q.device, q.dtype
         _heads("q", q, (torch.bfloat16, torch.float16), (None, None, None), dev)
         rows, qh, dim = q.shape
