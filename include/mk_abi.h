@@ -786,6 +786,8 @@ int mk_rotary_bind(MkModule* module, const MkRotaryBind* bind, MkLaunch** out);
 // sees up to kv_lens[b]: what lies elsewhere in the pool has no part in a result, and table entries of pages that lie wholly in
 // front may hold anything. Within those keys a NaN or infinity in a V row may reach rows that do not see its key (0 x NaN in the
 // product); in a K row it reaches the rows that see it. Page ids outside the pool are recorded (code 4) and read as zero rows.
+// cu_rows rises. Requests whose lengths contradict the extents are recorded and left out; all of them are where cu_rows[batch]
+// does, or where requests name more rows together than `rows`.
 typedef struct MkPrefixAttnBind {
     uint64_t q;            // bf16 or f16 [rows, q_heads, head_dim]
     int64_t q_row;         // strides in elements, multiples of 8

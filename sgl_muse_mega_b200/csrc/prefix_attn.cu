@@ -169,10 +169,11 @@ __device__ __forceinline__ Plan make_plan(const PrefixAttnArgs& a, const Lens& l
     Plan p;
     const int want = lens.want;
     p.tokens = lens.tokens;
-    int live = 0, ref = 0x7fffffff, lo = 0x7fffffff, hi = 0;
+    int live = 0, ref = 0x7fffffff, lo = 0x7fffffff, hi = 0, all = 0;
     lens.each(a, lane, [&](const Req& r, int b) {
         if (status != nullptr && b >= 32 * Lens::kHeld && b < a.batch)
             usable(a, b, __ldg(a.cu_rows + b), __ldg(a.cu_rows + b + 1), __ldg(a.kv_lens + b), status);  // to be recorded
+        all = min(all + r.n, 1 << 21);  // as far as it matters: a launch has up to 2^20 rows
         if (r.n > 0 && r.len > 0) {
             ++live;
             if (r.len >= want) ref = min(ref, b);
@@ -181,6 +182,11 @@ __device__ __forceinline__ Plan make_plan(const PrefixAttnArgs& a, const Lens& l
         }
         return true;
     });
+    // requests that name more rows than there are (where max_new lets them): their steps together could pass 32 bits, so nothing is done
+    if ((long long)a.batch * a.max_new > a.rows && (all = __reduce_add_sync(0xffffffffu, all)) > a.rows) {
+        if (status != nullptr && lane == 0) batch_status(status, 4, 525, all, a.rows);
+        return Plan{0, 0, 0, 0, 0, 0u, 0u, 0u, 0u};
+    }
     live = __reduce_add_sync(0xffffffffu, live);
     ref = __reduce_min_sync(0xffffffffu, ref);
     lo = __reduce_min_sync(0xffffffffu, lo);

@@ -187,3 +187,102 @@ def test_scores_far_from_zero(dt, length, step, sign, dim):
     op = c.launch()
     assert torch.isfinite(op.out).all() and op.status[0].item() == 0
     c.check(op)
+
+
+# ---- lengths that contradict the extents ------------------------------------------------------------------------------
+@pytest.mark.parametrize("change,out", [
+    (dict(kv_lens=[700, 1 << 20, 650]), [1]), (dict(kv_lens=[-1, 640, 650]), [0]), (dict(cu_rows=[0, 2, 6, 7]), [1]),
+    (dict(prefix_len=[-3]), []), (dict(prefix_len=[1 << 20]), []), (dict(cu_rows=[0, 2, 3, 9]), [0, 1, 2]),
+    (dict(cu_rows=[-2, 0, 3, 6]), [0]),
+])  # fmt: skip
+@pytest.mark.parametrize("dim", [64, 128])
+def test_lengths_that_contradict_the_extents(change, out, dim):
+    """A request left out keeps its rows as they were, the others are what they are."""
+    c = Batch(9, kv=[700, 640, 650], new=[2, 1, 3], prefix=384, qh=8, kvh=2, dim=dim, page=16, dt=BF)
+    cu = change.get("cu_rows", c.cu)
+    c.q = torch.cat((c.q, c.q[:1]))  # 7 rows
+    op = c.launch(**{k: dev(v, I32) for k, v in change.items()})
+    assert op.status[0].item() == 4
+    c.cu = [0, 2, 3, 6] if cu[3] > 7 else [max(x, 0) for x in cu]
+    rows = torch.zeros(7, dtype=torch.bool)
+    for b in range(3):
+        if b not in out:
+            rows[c.cu[b] : c.cu[b + 1]] = True
+    for b in out:  # the plain form takes no request that is left out
+        c.kv = [n if i != b else 0 for i, n in enumerate(c.kv)]
+    assert (op.out[~rows] == 5.0).all() and (op.lse[~rows.to(DEV)] == 5.0).all()
+    if rows.any():
+        c.check(op, rows)
+
+
+def test_requests_that_name_more_rows_than_there_are():
+    """Requests over and over on the same rows: nothing is done, and it is recorded. (Steps are counted in 32 bits, which the bind
+    provides for as far as requests share the rows out.)"""
+    B, rows, width = 4095, 256, 8192
+    lib = host.library()
+    q = torch.ones(rows, 8, 64, dtype=BF, device=DEV)
+    kv = torch.ones(128, 8, 64, dtype=BF, device=DEV)
+    cu = torch.zeros(B + 1, dtype=I32, device=DEV)
+    cu[1::2] = rows
+    op = BT.PrefixAttention(lib, lib.load(), q=q, k_cache=kv, v_cache=kv.clone(), block_table=torch.zeros(B, width, dtype=I32, device=DEV),
+                            kv_lens=torch.full((B,), width * 128, dtype=I32, device=DEV), cu_rows=cu, prefix_len=dev([0], I32), page_size=128,
+                            max_new=rows, scale=0.125)  # fmt: skip
+    op.out.fill_(5.0)
+    op.launch(stream())
+    torch.cuda.synchronize()
+    assert (op.out == 5.0).all() and op.status[:2].tolist() == [4, 520]  # the first to be recorded: every second request's rows
+
+
+# ---- a step's own tensors ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt,dim,page", [(BF, 64, 16), (HF, 128, 1), (HF, 64, 24)])
+def test_steps_on_the_pool_as_it_stands(dt, dim, page):
+    """Three captured steps of tables, rotation with append and attention: the attention against the rotated rows, pool and tables that
+    the launches in front of it left, so no rounding of theirs has to be allowed for."""
+    lib = host.library()
+    module = lib.load()
+    g = torch.Generator(device=DEV).manual_seed(12)
+    B, qh, kvh, prefix, rows = 5, 8, 2, 96, 24
+    width, pool = -(-200 // page), 7
+    n_pages = pool * width
+    ring = torch.randperm(n_pages, generator=g, device=DEV).int()
+    shared = prefix // page
+    r2p = torch.full((pool, width), -1, dtype=I32, device=DEV)
+    r2p[:, :shared] = ring[:shared]
+    owned = torch.full((pool,), shared, dtype=I32, device=DEV)
+    words = dev([shared, n_pages], I64)
+    kc, vc = (torch.full((n_pages * page, kvh, dim), math.nan, dtype=dt, device=DEV) for _ in range(2))
+    at = (ring[:shared, None].long() * page + torch.arange(page, device=DEV)).flatten()
+    kc[at], vc[at] = (torch.randn(len(at), kvh, dim, generator=g, device=DEV).to(dt) for _ in range(2))
+    lens = [shared * page] * B
+    seq, new, req = dev(lens, I64), dev([0] * B, I64), dev([3, 0, 6, 1, 4], I64)
+    tab = BT.BlockTables(lib, module, seq_lens=seq, new_lens=new, req_pool_indices=req, req_to_page=r2p, pages_owned=owned, free_pages=ring,
+                         free_words=words, page_size=page, rows=rows)  # fmt: skip
+    rope = BT.RopeTable(lib, module, rows=width * page, rot=dim, theta=5e5, device=DEV)
+    rope.launch(stream())
+    qkv = torch.zeros(rows, (qh + 2 * kvh) * dim, dtype=dt, device=DEV)
+    q, k, v = (t.unflatten(1, (-1, dim)) for t in qkv.split([qh * dim, kvh * dim, kvh * dim], 1))
+    rot = BT.Rotary(lib, module, q=q, k=k, v=v, positions=tab.positions, cos_sin_cache=rope.cos_sin, slots=tab.slots, k_cache=kc, v_cache=vc,
+                    n_rows=tab.cu_rows[B:], interleaved=True)  # fmt: skip
+    att = BT.PrefixAttention(lib, module, q=rot.q_out, k_cache=kc, v_cache=vc, block_table=tab.block_table, kv_lens=tab.kv_lens,
+                             cu_rows=tab.cu_rows, prefix_len=dev([shared * page], I32), page_size=page, max_new=8, scale=0.125, lse=True)  # fmt: skip
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        for op in (tab, rot, att):
+            op.launch(stream(), True)
+    c = Batch.__new__(Batch)
+    c.k, c.v, c.page, c.window, c.dt = kc, vc, page, 0, dt
+    for take in ([8, 1, 3, 5, 7], [1, 0, 8, 2, 1], [4, 4, 1, 8, 6]):
+        new.copy_(dev(take, I64))
+        qkv.copy_(torch.randn(qkv.shape, generator=g, device=DEV))
+        att.out.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(op.status[0].item() == 0 for op in (tab, rot, att))
+        c.q, c.table, c.kv, c.cu = rot.q_out, tab.block_table.cpu(), tab.kv_lens.tolist(), tab.cu_rows.tolist()
+        n = sum(take)
+        assert c.cu[-1] == n and c.kv == [a + b for a, b in zip(lens, take)] and (att.out[n:] == 5.0).all()
+        c.check(att, slice(0, n))
+        lens = c.kv
+        seq.copy_(dev(lens, I64))
+    graph.reset()
