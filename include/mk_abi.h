@@ -790,7 +790,7 @@ int mk_rotary_bind(MkModule* module, const MkRotaryBind* bind, MkLaunch** out);
 // does, or where requests name more rows together than `rows`.
 typedef struct MkPrefixAttnBind {
     uint64_t q;            // bf16 or f16 [rows, q_heads, head_dim]
-    int64_t q_row;         // strides in elements, multiples of 8
+    int64_t q_row;         // strides in elements, multiples of 8; rows behind one another, with their heads inside
     int64_t q_head;
     uint64_t k_cache;      // [kv_rows, kv_heads, head_dim]
     int64_t k_row;

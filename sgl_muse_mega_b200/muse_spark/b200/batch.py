@@ -50,7 +50,7 @@ def _heads(name: str, t: torch.Tensor, dtype, shape, device):
     if t.numel() and t.stride(2) != 1:
         raise ValueError(f"{name}: the last dimension is strided")
     if t.shape[0] > 1 and t.stride(0) < (t.shape[1] - 1) * t.stride(1) + t.shape[2]:
-        raise ValueError(f"{name}: rows overlap")
+        raise ValueError(f"{name}: rows overlap, or do not hold their heads (heads outermost)")
     if t.shape[1] > 1 and t.stride(1) < t.shape[2]:
         raise ValueError(f"{name}: heads overlap")
 

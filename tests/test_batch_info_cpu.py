@@ -1,5 +1,7 @@
-"""What the batched step's launches say of themselves without a GPU: grid, block and shared memory as they are launched."""
+"""The batched step's launches without a GPU: what they say of themselves (grid, block and shared memory as they are launched), and what
+the C binds refuse that the Python classes never ask for."""
 
+import pytest
 import torch
 
 from sgl_muse_mega_b200.common import host
@@ -58,3 +60,28 @@ def test_prefix_attention():
     assert shape(op(4, 4, 128)) == (2, 148, 384, 7 * 32768 + 1024, 1)
     assert shape(op(500, 16, 64)) == (2, 1000, 384, 12 * 16384 + 1024, 1)
     assert shape(op(5000, 16, 64)) == (2, 12 * 148, 384, 12 * 16384 + 1024, 1)
+
+
+@pytest.mark.parametrize("over,msg", [
+    (dict(k_row=64), "k_cache: row stride"), (dict(v_row=64, v_head=64 * 64), "v_cache: row stride"), (dict(k_head=0), "k_cache: head stride"),
+    (dict(q_head=32), "q: head stride"), (dict(q_row=64, q_head=4 * 64), "q: row stride"), (dict(q_row=0), "q: row stride"), (dict(k_row=0), "k_cache: row stride"),
+    (dict(q_head=0), "head stride"), (dict(k_row=136), None), (dict(q_row=512, q_head=128), None),
+])  # fmt: skip
+def test_prefix_attention_strides(over, msg):
+    """Heads-outermost pools and rows inside one another have no tensor map."""
+    lib = host.library()
+    op = BT.PrefixAttention(lib, None, q=z(4, 4, 64, dtype=BF), k_cache=z(64, 2, 64, dtype=BF), v_cache=z(64, 2, 64, dtype=BF), block_table=z(2, 4),
+                            kv_lens=z(2), cu_rows=z(3), prefix_len=z(1), page_size=16, max_new=2, scale=0.125)  # fmt: skip
+    for name, value in over.items():
+        setattr(op.bind, name, value)
+    if msg is None:
+        lib.bind("mk_prefix_attn_bind", None, op.bind)
+        return
+    with pytest.raises(RuntimeError, match=msg):
+        lib.bind("mk_prefix_attn_bind", None, op.bind)
+
+
+def test_heads_outermost_is_refused():
+    with pytest.raises(ValueError, match="heads outermost"):
+        BT.PrefixAttention(host.library(), None, q=z(4, 4, 64, dtype=BF), k_cache=z(2, 64, 64, dtype=BF).transpose(0, 1), v_cache=z(64, 2, 64, dtype=BF),
+                           block_table=z(2, 4), kv_lens=z(2), cu_rows=z(3), prefix_len=z(1), page_size=16, max_new=2, scale=0.125)  # fmt: skip
