@@ -85,3 +85,14 @@ def test_heads_outermost_is_refused():
     with pytest.raises(ValueError, match="heads outermost"):
         BT.PrefixAttention(host.library(), None, q=z(4, 4, 64, dtype=BF), k_cache=z(2, 64, 64, dtype=BF).transpose(0, 1), v_cache=z(64, 2, 64, dtype=BF),
                            block_table=z(2, 4), kv_lens=z(2), cu_rows=z(3), prefix_len=z(1), page_size=16, max_new=2, scale=0.125)  # fmt: skip
+
+
+@pytest.mark.parametrize("scaling", [
+    dict(kind="linear", factor=1e-310), dict(kind="ntk", factor=1e300), dict(kind="ntk", factor=1e-320),
+    dict(kind="llama3", factor=1e-310, low_freq_factor=1.0, high_freq_factor=4.0, original_len=1),  # a sixth of a turn: all scaled
+    dict(kind="yarn", factor=1e-310, beta_fast=32.0, beta_slow=1.0, original_len=8192),
+])  # fmt: skip
+def test_rope_table_whose_frequencies_are_not_numbers(scaling):
+    """A table of NaN, or of cos 0 throughout, is no table."""
+    with pytest.raises(RuntimeError, match="factor"):
+        BT.RopeTable(host.library(), None, rows=5, rot=8, theta=1e4, device="cpu", scaling=scaling)
