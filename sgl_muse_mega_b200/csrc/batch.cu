@@ -17,8 +17,8 @@ namespace mk {
 // the whole batch into shared memory (24 bytes a request; two dependent round trips to L2), then fills its share of the
 // table entries and rows. Table entries below owned_b come from the request's own row, the others straight from the ring,
 // so no CTA reads what another writes. The two words that every CTA reads and the launch advances (pages owned, ring
-// head) are written by the CTA that arrives last, after all have read them. One request: 5.4 us inside a graph, 256 requests x 2064
-// pages (3.2 MB): 6.9 us, bound by those dependent loads.
+// head) are written by the CTA that arrives last, after all have read them. One request: 5.2 us inside a graph, 256 requests x 2064
+// pages (3.2 MB): 6.8 us, bound by those dependent loads; 7.8 and 8.5 a call on a stream.
 struct TablesShared {
     int *seq, *cu, *off, *own, *need, *row;
     unsigned *seen, *twice;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Bloc
 // in 32. A 64-bit sine pair costs about a hundred double operations, so a thread evaluates it once for kRows positions of a
 // frequency and turns on from one position to the next by the addition theorem with the pair of a single step (from the
 // host): four double operations a pair, error at most kRows 2^-52 against the 2^-24 of the result's own rounding. 131,072 x 128
-// (67 MB): 13.3 us, 5.1 TB/s of stores; 8,448 x 64: 2.4 us, one thread's chain.
+// (67 MB): 15.1 us a table of three in turn, 4.4 TB/s of stores; 8,448 x 64: 2.5 us, one thread's chain.
 template <int kRows>
 __global__ void __launch_bounds__(128) rope_table_kernel(const RopeTableArgs a) {
     const int F = a.rot / 2, groups = F / 4;  // a thread: four neighbouring frequencies of kRows positions

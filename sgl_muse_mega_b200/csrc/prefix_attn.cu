@@ -20,10 +20,11 @@
 // rows, or gathers of four rows where pages are small or odd). Steps alternate between the two warpgroups, each with its
 // own S, P and O in tensor memory: while one takes the exponentials of its step the tensor core works for the other.
 //
-// Measured (whole launch, both kernels): 32 requests x 16 rows over 32 K shared tokens, 16 heads of 64 on 2 kv heads: 121 us = 574 TFLOP/s,
-// bound by the softmax's phases that depend on one another (two steps a CTA take about 3000 cycles, their exponentials 2 x 900 of
-// those, their products 920); 96 requests over 2 K tokens of their own, 64 heads of 128 on 8: 154 us = 5.3 TB/s, DRAM and power;
-// 64 requests behind 8 K shared tokens 27 us, one request of 16 rows over a window of 2047 keys 18.6 us: latency.
+// Measured (both kernels, a pass inside a CUDA graph; passes on a stream take 1.5 - 2.5 us more): 32 requests x 16 rows over 32 K shared
+// tokens, 16 heads of 64 on 2 kv heads: 121 us = 572 TFLOP/s, bound by the softmax's phases that depend on one another (two steps a CTA
+// take about 3300 cycles; a warp's two halves of exponentials 740 + 950 of them, the unit they go through 2000 for both, the products 920);
+// 96 requests over 2 K tokens of their own, 64 heads of 128 on 8: 153 us = 5.4 TB/s, DRAM, in a long run 163 - 176 at the board's power
+// limit; 64 requests behind 8 K shared tokens 26 us, one request of 16 rows over a window of 2047 keys 17 us: latency.
 #include "batch.h"
 #include "umma.cuh"
 #include "util.cuh"
