@@ -286,3 +286,33 @@ def test_steps_on_the_pool_as_it_stands(dt, dim, page):
         lens = c.kv
         seq.copy_(dev(lens, I64))
     graph.reset()
+
+
+# ---- long rows, rows that see a NaN -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_a_million_keys(dt):
+    """Against outputs of a few hundredths, with the bound of every other case."""
+    c = Batch(10, kv=[1000003], new=[2], prefix=0, qh=2, kvh=1, dim=64, page=128, dt=dt, q_std=3.0)
+    c.check(c.launch())
+
+
+@pytest.mark.parametrize("dim,window", [(64, 0), (64, 200), (128, 0)])
+def test_a_nan_in_a_key_reaches_the_rows_that_see_it(dim, window):
+    """The second of a request's four new keys, and a shared key that some windows have left behind."""
+    c = Batch(11, kv=[700, 640, 650], new=[4, 1, 2], prefix=512, qh=8, kvh=2, dim=dim, page=16, dt=BF, window=window)
+    shared = 490  # in front of what the first request's rows see through a window of 200 (496 and on), not of what the others' see
+    at = [(0, 697)] + [(b, shared) for b in range(3)]
+    for b, key in at:
+        c.k[c.slots(b, [key])] = math.nan
+    op = c.launch()
+    hit = torch.zeros(7, dtype=torch.bool)
+    hit[1:4] = True
+    if window == 0:
+        hit[:] = True
+    else:
+        hit[4:] = True
+    assert torch.equal(op.out.isnan().flatten(1).all(1).cpu(), hit) and torch.equal(op.out.isnan().flatten(1).any(1).cpu(), hit)
+    for b, key in at:  # the plain form multiplies by zero too
+        c.k[c.slots(b, [key])] = 0.0
+    if window:
+        c.check(op, ~hit)
